@@ -225,6 +225,71 @@ int prism_codec_pass(prism_ctx* ctx, int kind, const int32_t* push, int n_push,
  * wait of a per-pass kernel gives up: PRISM_E_TIMEOUT, else PRISM_OK. */
 int prism_ctx_status(prism_ctx* ctx, void* stream);
 
+/* ---- the trainable pre-norm gated feed-forward sub-block ---------------------------
+ * No counterpart in the reference (its shaders only infer, and none normalises, gates or
+ * drops out).  Three operators and their backward passes, for training or fine-tuning the
+ * feed-forward half of a block and for serving it:
+ *     n = layer_norm(x);  h = gated_ffn(n);  y = x + dropout(h)
+ * The caller owns every tensor: raw device pointers, rows of `dim` values that are
+ * consecutive in memory, rows at *_stride ELEMENTS from one another (at least dim; ignored
+ * for a single row), so column slices of a wider buffer work.  Activations, weights and
+ * gradients are fp16, bf16 or fp32 (enum prism_dtype); sums and statistics are fp32.
+ * Scratch memory is the caller's too: *_workspace() says how many bytes a call with these
+ * params needs (16-byte aligned, any contents, free again when the call's work has run), so
+ * calls on different streams, threads or captured graphs share nothing unless the caller
+ * gives them the same workspace.  The same inputs give the same bits (no atomics).
+ * Calls are stream-ordered, never synchronise, never allocate and can be captured into a
+ * CUDA graph.  rows == 0 is a no-op (the gradients of parameters become zero). */
+enum prism_dtype { PRISM_DTYPE_F16 = 0, PRISM_DTYPE_BF16 = 1, PRISM_DTYPE_F32 = 2 };
+
+/* dtype: x, y, dy, add, dx.  param_dtype: weight, bias, dweight, dbias; dtype or fp32.
+ * 1 <= dim <= 16384.  Rows whose bases and strides are multiples of 16 bytes are read in
+ * 16-byte accesses; others work, more slowly. */
+typedef struct prism_norm_params {
+    int64_t rows;
+    int64_t x_stride, y_stride, dy_stride, add_stride, dx_stride;
+    int32_t dim;
+    int32_t dtype, param_dtype;
+    float eps;
+} prism_norm_params;
+
+/* y = (x - mean) * rstd * weight + bias with mean and rstd = 1/sqrt(variance + eps) over each
+ * row's dim values.  weight (nullable: ones), bias (nullable: zeros): [dim].  mean, rstd
+ * (nullable): fp32 [rows], what the backward pass needs.  y may be x itself. */
+int prism_layer_norm(prism_ctx* ctx, const prism_norm_params* p, const void* x, const void* weight,
+                     const void* bias, void* y, float* mean, float* rstd, void* stream);
+
+/* With xh = (x - mean) * rstd and g = dy * weight:
+ *     dx = rstd * (g - mean_c(g) - xh * mean_c(g * xh)) + add
+ *     dweight = sum over rows of dy * xh,   dbias = sum over rows of dy
+ * add (nullable): the gradient that reached x past the norm (the residual path).  dweight,
+ * dbias (nullable): overwritten.  The workspace is needed if either is wanted.  dx may be x,
+ * dy or add itself. */
+int prism_layer_norm_backward(prism_ctx* ctx, const prism_norm_params* p, const void* x, const void* weight,
+                              const float* mean, const float* rstd, const void* dy, const void* add, void* dx,
+                              void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+int prism_layer_norm_backward_workspace(prism_ctx* ctx, const prism_norm_params* p, size_t* bytes);
+
+/* dtype: x, residual, y.  threshold: of 65536; an element is dropped with probability
+ * threshold / 65536 (0 .. 65535) and scaled by 65536 / (65536 - threshold) otherwise. */
+typedef struct prism_dropout_params {
+    int64_t rows;
+    int64_t x_stride, residual_stride, y_stride;
+    int32_t dim;
+    int32_t dtype;
+    int32_t threshold;
+} prism_dropout_params;
+
+/* y = residual + (kept ? x * scale : 0); residual nullable.  The mask is never stored: it is a
+ * function of rng = {seed, offset} (two uint64 in DEVICE memory, read when the call runs, so a
+ * replayed graph draws a new mask once they have changed) and of the element's index
+ * i = row * dim + column: bits 16 (i mod 8) .. + 15 of the 128 bits (word 0 first, low half
+ * first) of the Philox4x32-10 block with counter (i / 8, offset) and key seed, low words first;
+ * the element is kept iff they are >= threshold.  The backward pass is the same call on the
+ * gradient with the same rng and threshold and no residual.  y may be x or residual itself. */
+int prism_dropout_add(prism_ctx* ctx, const prism_dropout_params* p, const void* x, const void* residual,
+                      const uint64_t* rng, void* y, void* stream);
+
 /* ---- fast path: a whole stack over a batch of frames ------------------------ */
 
 enum prism_block_kind { PRISM_BLOCK_MOE = 0, PRISM_BLOCK_DENSE = 1 };

@@ -2,13 +2,15 @@
 transformer / MoE stack behind the C ABI of include/prism_moe.h.
 
 The Python layer is a thin host mirror over libprism_moe.so (ctypes): PyTorch is
-used only to own device memory and streams.  Two interfaces:
+used only to own device memory and streams.  Three interfaces:
 
 * the per-pass drop-ins, one call per reference vkCmdDispatch, taking the same
   push-constant blocks (AttnParams, RouterParams, ExpertParams, ProjParams,
   DenseParams) and the three arenas (fp16 weight blob, fp16 feature arena, int32 aux
   arena) - the dispatch contract of prism_moe_bench.cpp:213-505;
-* Stack: the whole stack of a StackLayout over a batch of frames (the fast path).
+* Stack: the whole stack of a StackLayout over a batch of frames (the fast path);
+* the trainable pre-norm gated feed-forward sub-block on the caller's own tensors: layer_norm,
+  gated_ffn, dropout_add and their backward passes (methods of Prism).
 
 No entry point falls back to the CPU: a missing libprism_moe.so raises.
 """
@@ -17,8 +19,8 @@ from __future__ import annotations
 import ctypes as C
 
 from . import abi, configs, layout, synth
-from .abi import (AttnParams, DenseParams, ExpertParams, PrismError, ProjParams, RouterParams,
-                  check)
+from .abi import (AttnParams, DenseParams, DropoutParams, ExpertParams, NormParams, PrismError, ProjParams,
+                  RouterParams, check)
 from .layout import StackLayout, build_stack
 
 __all__ = ["Prism", "Stack", "AttnParams", "RouterParams", "ExpertParams", "ProjParams",
@@ -47,6 +49,73 @@ def _stream(stream) -> int | None:
         import torch
         return torch.cuda.current_stream().cuda_stream
     return getattr(stream, "cuda_stream", stream)
+
+
+_DTYPES = {}  # torch dtype -> prism_dtype
+
+
+def _dtype(t, name: str) -> int:
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({getattr(torch, d): i for i, d in enumerate(abi.DTYPES)})
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{name}: dtype {t.dtype} (fp16, bf16 or fp32)") from None
+
+
+def _rows(t, name: str, like=None):
+    """(rows, dim, row stride) of a tensor [..., dim] whose last dimension is consecutive in memory;
+    `like` = (tensor, rows, dim) it must match in type, device, rows and dim."""
+    if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: the last dimension is not consecutive in memory")
+    dim = t.shape[-1]
+    if t.dim() == 2:
+        rows, stride = t.shape[0], t.stride(0)
+    else:
+        rows, stride = t.numel() // max(1, dim), dim
+        if not t.is_contiguous():
+            try:
+                stride = t.view(-1, dim).stride(0)
+            except RuntimeError:
+                raise ValueError(f"{name}: its rows do not lie at one stride") from None
+    if rows <= 1:
+        stride = dim
+    if like is not None:
+        ref, r, d = like
+        if t.dtype != ref.dtype or t.device != ref.device or rows != r or dim != d:
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device} beside {ref.dtype} [{r}, {d}] on {ref.device}")
+    return rows, dim, stride
+
+
+def _flat(t, name: str, shape, dtype, device) -> int | None:
+    """Address of a contiguous parameter, gradient or statistics tensor; None passes through."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _workspace(workspace, nbytes: int, device, stream):
+    """(tensor, address, bytes): the caller's workspace, or one from torch's allocator that belongs to
+    the call's stream (so it is not handed out again before the call's work has run)."""
+    if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace: expected a contiguous tensor on {device}")
+        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if not nbytes:
+        return None, None, 0
+    import torch
+    if stream is None:
+        w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        if not hasattr(stream, "cuda_stream"):
+            stream = torch.cuda.ExternalStream(stream, device=device)
+        with torch.cuda.stream(stream):
+            w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return w, w.data_ptr(), nbytes
 
 
 class Prism:
@@ -115,6 +184,84 @@ class Prism:
                                                   _ptr(weights), weights.numel(), _ptr(features), features.numel(),
                                                   _ptr(rgb) if rgb is not None else None,
                                                   rgb.numel() if rgb is not None else 0, _stream(stream)))
+
+    # ---- the trainable pre-norm gated feed-forward sub-block (caller-owned CUDA tensors) ----
+    # Tensors are [..., dim] with the last dimension consecutive and the rows at one stride (column
+    # slices of wider buffers work); the caller allocates outputs.  stream: None = torch's current
+    # stream of the context's device; tensors made on another stream are the caller's to order.
+    # workspace: scratch memory of at least the *_workspace() bytes, None = from torch's allocator.
+    def _on_device(self, t, name: str):
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{name}: on {t.device}, the context is for cuda:{self.device}")
+
+    def _stream(self, stream):
+        if stream is None:
+            import torch
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return getattr(stream, "cuda_stream", stream)
+
+    @staticmethod
+    def _param_dtype(ps, x):
+        """dtype of the norm's parameters: the first given one's (fp32 or the rows' own), else the rows'."""
+        for p in ps:
+            if p is not None:
+                return p.dtype, _dtype(p, "weight")
+        return x.dtype, _dtype(x, "x")
+
+    def layer_norm(self, x, weight, bias, y, eps: float = 1e-5, mean=None, rstd=None, stream=None):
+        """prism_layer_norm: y = (x - mean) * rstd * weight + bias over the last dimension.  weight, bias
+        ([dim], x's dtype or fp32) and the fp32 statistics mean, rstd ([rows]) are optional."""
+        import torch
+        self._on_device(x, "x")
+        rows, dim, xs = _rows(x, "x")
+        ys = _rows(y, "y", (x, rows, dim))[2]
+        pt, pcode = self._param_dtype((weight, bias), x)
+        p = NormParams(rows=rows, x_stride=xs, y_stride=ys, dim=dim, dtype=_dtype(x, "x"), param_dtype=pcode, eps=eps)
+        check(self.lib, self.lib.prism_layer_norm(
+            self.h, C.byref(p), _ptr(x), _flat(weight, "weight", (dim,), pt, x.device),
+            _flat(bias, "bias", (dim,), pt, x.device), _ptr(y), _flat(mean, "mean", (rows,), torch.float32, x.device),
+            _flat(rstd, "rstd", (rows,), torch.float32, x.device), self._stream(stream)))
+        return y
+
+    def layer_norm_backward(self, x, weight, mean, rstd, dy, dx, dweight=None, dbias=None, add=None, workspace=None,
+                            stream=None):
+        """prism_layer_norm_backward: dx (+ add, the gradient that came past the norm), and the parameters'
+        gradients where dweight, dbias are given (overwritten)."""
+        import torch
+        self._on_device(x, "x")
+        rows, dim, xs = _rows(x, "x")
+        like = (x, rows, dim)
+        pt, pcode = self._param_dtype((weight, dweight, dbias), x)
+        p = NormParams(rows=rows, x_stride=xs, dy_stride=_rows(dy, "dy", like)[2], dx_stride=_rows(dx, "dx", like)[2],
+                       add_stride=_rows(add, "add", like)[2] if add is not None else 0, dim=dim, dtype=_dtype(x, "x"),
+                       param_dtype=pcode)
+        need = C.c_size_t()
+        if dweight is not None or dbias is not None:
+            check(self.lib, self.lib.prism_layer_norm_backward_workspace(self.h, C.byref(p), C.byref(need)))
+        keep, ws, ws_bytes = _workspace(workspace, need.value, x.device, stream)
+        check(self.lib, self.lib.prism_layer_norm_backward(
+            self.h, C.byref(p), _ptr(x), _flat(weight, "weight", (dim,), pt, x.device),
+            _flat(mean, "mean", (rows,), torch.float32, x.device), _flat(rstd, "rstd", (rows,), torch.float32, x.device),
+            _ptr(dy), _ptr(add) if add is not None else None, _ptr(dx),
+            _flat(dweight, "dweight", (dim,), pt, x.device), _flat(dbias, "dbias", (dim,), pt, x.device), ws, ws_bytes,
+            self._stream(stream)))
+        return dx
+
+    def dropout_add(self, x, residual, y, p: float, rng, stream=None):
+        """prism_dropout_add: y = residual + dropout(x) (residual None: dropout(x)), dropping with probability
+        round(65536 p) / 65536.  rng: CUDA int64 [2] {seed, offset}, read when the call runs.  The gradient:
+        the same call on it, with the same p and rng and no residual."""
+        import torch
+        self._on_device(x, "x")
+        rows, dim, xs = _rows(x, "x")
+        like = (x, rows, dim)
+        q = DropoutParams(rows=rows, x_stride=xs, y_stride=_rows(y, "y", like)[2],
+                          residual_stride=_rows(residual, "residual", like)[2] if residual is not None else 0, dim=dim,
+                          dtype=_dtype(x, "x"), threshold=max(-1, min(65536, int(round(65536 * p)))))
+        check(self.lib, self.lib.prism_dropout_add(
+            self.h, C.byref(q), _ptr(x), _ptr(residual) if residual is not None else None,
+            _flat(rng, "rng", (2,), torch.int64, x.device), _ptr(y), self._stream(stream)))
+        return y
 
     def status(self, stream=None):
         """prism_ctx_status: raises PrismError if a per-pass kernel's bounded wait gave up."""

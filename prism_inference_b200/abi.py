@@ -62,6 +62,16 @@ class StackDesc(C.Structure):
                        "out_dim down_w down_b n_blocks") + [("blocks", C.POINTER(BlockDesc))]
 
 
+class NormParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in "rows x_stride y_stride dy_stride add_stride dx_stride".split()] + \
+        _fields("dim dtype param_dtype") + [("eps", C.c_float)]
+
+
+class DropoutParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in "rows x_stride residual_stride y_stride".split()] + \
+        _fields("dim dtype threshold")
+
+
 def stack_desc(L: StackLayout):
     """(StackDesc, keep-alive block array) for a StackLayout."""
     arr = (BlockDesc * max(1, len(L.blocks)))()
@@ -88,11 +98,14 @@ EXPORTS = ("prism_create", "prism_destroy", "prism_last_error_string", "prism_ab
            "prism_stack_tokens_per_frame", "prism_stack_profile", "prism_stack_profile_read", "prism_stack_set_option",
            "prism_expert_all_static", "prism_stack_inject_stall", "prism_stack_infer",
            "prism_stack_submit", "prism_stack_wait", "prism_moe_block", "prism_stack_infer_gpu",
-           "prism_codec_pass", "prism_ctx_status")
+           "prism_codec_pass", "prism_ctx_status", "prism_layer_norm", "prism_layer_norm_backward",
+           "prism_layer_norm_backward_workspace", "prism_dropout_add")
 # prism_codec_kind order = the shaders of oracle.CODEC_KINDS
 CODEC_KINDS = ("conv3x3_coopvec_9ch", "strided_conv_coopvec_32ch", "strided_conv_split_64ch",
                "strided_conv_split_128ch", "dec3_fused", "dec2_fused", "dec1_fused",
                "pw_conv_coopvec_32to12", "pixelshuffle_sigmoid")
+# prism_dtype
+DTYPES = ("float16", "bfloat16", "float32")
 STATIC_MAX_TOKENS = 65536  # PRISM_STATIC_MAX_TOKENS
 # prism_stack_option
 OPT_PAIR_ATTENTION = 1
@@ -143,6 +156,10 @@ def load(path: os.PathLike | None = None) -> C.CDLL:
         "prism_stack_set_option": (i32, [vp, i32, i32]),
         "prism_expert_all_static": (i32, [vp, C.POINTER(ExpertParams), C.c_int32, C.c_int32, vp, sz, vp, sz, vp,
                                           sz, vp]),
+        "prism_layer_norm": (i32, [vp, C.POINTER(NormParams), vp, vp, vp, vp, vp, vp, vp]),
+        "prism_layer_norm_backward": (i32, [vp, C.POINTER(NormParams)] + [vp] * 10 + [sz, vp]),
+        "prism_layer_norm_backward_workspace": (i32, [vp, C.POINTER(NormParams), C.POINTER(sz)]),
+        "prism_dropout_add": (i32, [vp, C.POINTER(DropoutParams), vp, vp, vp, vp, vp]),
         "prism_stack_profile_read": (i32, [vp, C.POINTER(C.c_double), C.POINTER(C.c_int64), i32]),
     }
     for name, (res, args) in sig.items():

@@ -1,0 +1,133 @@
+"""Plain 64-bit forms of the trainable sub-block's operators, written from their formulas, with the
+tolerances of their fp32 arithmetic.
+
+A tolerance is counted in roundings.  U32 = 2^-24 is one fp32 rounding; u(dtype) = eps / 2 is the one
+rounding of an output to its type.  A sum of n terms in fp32 is off by at most (its longest chain of
+additions) * U32 * (the sum of the terms' magnitudes)."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+U32 = 2.0 ** -24
+M32 = 0xFFFFFFFF
+# the smallest spacing of each type below its normal range (subnormal results are off by half of it)
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check(got, want, tol, what):
+    """|got - want| <= u |want| + tol, element by element; infinities and NaN in the same places."""
+    got64, want = got.double().cpu(), want.cpu()
+    tol = tol.cpu() if torch.is_tensor(tol) else torch.full_like(want, tol)
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(want), torch.isnan(got64)), f"{what}: NaN in other places"
+    same_inf = want[torch.isinf(want)] == got64[torch.isinf(want)]
+    assert same_inf.all(), f"{what}: infinities in other places"
+    # the value before its rounding is off by tol, so its own rounding is half a step of |want| + tol
+    bound = tol + u(got.dtype) * (want.abs() + tol) + TINY[got.dtype]
+    off = (got64 - want).abs()
+    bad = fin & ~(off <= bound)
+    if bad.any():
+        i = (off / bound).masked_fill(~bad, 0).argmax()
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off; worst at {int(i)}: got "
+                             f"{got64.reshape(-1)[i]:.9g}, want {want.reshape(-1)[i]:.9g}, bound {bound.reshape(-1)[i]:.3g}")
+
+
+# ---- layer norm -----------------------------------------------------------------------------
+# A thread adds at most 64 of its own values, then at most 5 lanes and 8 warps: 77 additions, and a
+# few roundings on each value: 96 in all.
+K_ROW = 96
+
+
+def norm(x, w, b, eps):
+    """(y, mean, rstd) and their tolerances."""
+    x, D = x.double(), x.shape[-1]
+    w = torch.ones(D, dtype=torch.float64, device=x.device) if w is None else w.double()
+    b = torch.zeros(D, dtype=torch.float64, device=x.device) if b is None else b.double()
+    mean = x.mean(-1)
+    c = x - mean[:, None]
+    var = (c * c).mean(-1)
+    rstd = 1 / torch.sqrt(var + eps)
+    y = c * rstd[:, None] * w + b
+    t_mean = K_ROW * U32 * x.abs().mean(-1)
+    t_c = t_mean[:, None] + U32 * c.abs()  # x - mean
+    # the second moment: its own additions and twice the error of the centred values
+    t_var = (K_ROW * U32 * (c * c) + 2 * c.abs() * t_c + t_c * t_c).mean(-1)
+    t_rstd = rstd * (0.5 * t_var / (var + eps) + 4 * U32)
+    t_y = w.abs() * (t_c * rstd[:, None] + c.abs() * t_rstd[:, None]) + 4 * U32 * ((c * rstd[:, None] * w).abs() + b.abs())
+    return (y, mean, rstd), (t_y, t_mean, t_rstd)
+
+
+def norm_back(x, w, mean, rstd, dy, add):
+    """(dx, dweight, dbias) and their tolerances, from the given statistics."""
+    x, dy, R, D = x.double(), dy.double(), x.shape[0], x.shape[-1]
+    w = torch.ones(D, dtype=torch.float64, device=x.device) if w is None else w.double()
+    m, r = mean.double()[:, None], rstd.double()[:, None]
+    xh, g = (x - m) * r, dy * w
+    t_xh = 3 * U32 * (x.abs() + m.abs()) * r.abs()
+    m0, m1 = g.mean(-1, keepdim=True), (g * xh).mean(-1, keepdim=True)
+    t_m0 = K_ROW * U32 * g.abs().mean(-1, keepdim=True)
+    t_m1 = (K_ROW * U32 * (g * xh).abs() + g.abs() * t_xh).mean(-1, keepdim=True)
+    dx = r * (g - m0 - xh * m1)
+    t_dx = r.abs() * (t_m0 + t_xh * m1.abs() + xh.abs() * t_m1 + 6 * U32 * (g.abs() + m0.abs() + (xh * m1).abs()))
+    if add is not None:
+        dx = dx + add.double()
+        t_dx = t_dx + 2 * U32 * (add.double().abs() + dx.abs())
+    # rows one after the other in a thread (at least 296 threads a column once there are that many
+    # rows, 2 CTAs on each of 148 SMs), then teams, warps and partial sums
+    k = R / 296 + 1 + 64
+    dw, db = (dy * xh).sum(0), dy.sum(0)
+    t_dw = k * U32 * (dy * xh).abs().sum(0) + (dy.abs() * t_xh).sum(0)
+    t_db = k * U32 * dy.abs().sum(0)
+    return (dx, dw, db), (t_dx, t_dw, t_db)
+
+
+# ---- dropout ----------------------------------------------------------------------------------
+
+
+def philox_block(counter, key):
+    """One Philox4x32-10 block in Python integers (Salmon, Moraes, Dror, Shaw, 2011)."""
+    c, k = list(counter), list(key)
+    for _ in range(10):
+        a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(b >> 32) ^ c[1] ^ k[0], b & M32, (a >> 32) ^ c[3] ^ k[1], a & M32]
+        k = [(k[0] + 0x9E3779B9) & M32, (k[1] + 0xBB67AE85) & M32]
+    return c
+
+
+def draws(rng, n):
+    """The 16-bit draws of elements 0 .. n - 1."""
+    seed, off = int(rng[0]), int(rng[1])
+    out = []
+    for i in range((n + 7) // 8):
+        for word in philox_block([i & M32, i >> 32, off & M32, (off >> 32) & M32], [seed & M32, (seed >> 32) & M32]):
+            out += [word & 0xFFFF, word >> 16]
+    return torch.tensor(out[:n], dtype=torch.int64)
+
+
+def dropout(x, residual, threshold, rng):
+    x = x.double().cpu()
+    keep = (draws(rng, x.numel()) >= threshold).reshape(x.shape)
+    v = torch.where(keep, x * (65536 / (65536 - threshold)), torch.zeros_like(x))
+    y = v if residual is None else v + residual.double().cpu()
+    return y, 4 * U32 * (v.abs() + y.abs()), keep
+
+
+# ---- the gated feed-forward block ------------------------------------------------------------
+
+
+def act(g, kind):
+    """act(g), its first derivative, and bounds of the first and second derivatives' magnitudes."""
+    if kind == "relu":
+        return g.clamp(min=0), (g > 0).double()
+    if kind == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    c, a = math.sqrt(2 / math.pi), 0.044715
+    s = torch.sigmoid(2 * c * (g + a * g ** 3))
+    return g * s, s + g * s * (1 - s) * 2 * c * (1 + 3 * a * g * g)
