@@ -290,6 +290,44 @@ typedef struct prism_dropout_params {
 int prism_dropout_add(prism_ctx* ctx, const prism_dropout_params* p, const void* x, const void* residual,
                       const uint64_t* rng, void* y, void* stream);
 
+/* The gate's activation.  GELU is the tanh form that the framework's other blocks use. */
+enum prism_activation { PRISM_ACT_GELU = 0, PRISM_ACT_SILU = 1, PRISM_ACT_RELU = 2 };
+
+/* dtype: every tensor of the call, fp16 or bf16.  dim and hidden: multiples of 8, at most 16384
+ * and 65536.  Row tensors and weights start on 16-byte boundaries, strides are multiples of 8. */
+typedef struct prism_gated_params {
+    int64_t rows;
+    int64_t x_stride, residual_stride, y_stride, dy_stride, dx_stride;
+    int32_t dim, hidden;
+    int32_t dtype, activation;
+} prism_gated_params;
+
+/* w_gate, w_up: [hidden][dim], w_down: [dim][hidden], row-major and contiguous as everywhere in
+ * this header; b_gate, b_up [hidden] and b_down [dim] are nullable (zeros). */
+typedef struct prism_gated_weights {
+    const void *w_gate, *b_gate, *w_up, *b_up, *w_down, *b_down;
+} prism_gated_weights;
+/* Gradients, laid out as the weights; overwritten; each nullable. */
+typedef struct prism_gated_grads {
+    void *dw_gate, *db_gate, *dw_up, *db_up, *dw_down, *db_down;
+} prism_gated_grads;
+
+/* y = w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down + residual, row by row; residual
+ * nullable.  Products accumulate in fp32; the hidden values are rounded once to dtype, as the
+ * operand of the last product, and y once.  y must not overlap x; it may be residual itself. */
+int prism_gated_ffn(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
+                    const void* residual, void* y, void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients of sum(dy * y) without the residual path (dy itself) from x and the weights: the
+ * forward pass keeps nothing, the gate and up projections are computed again (in fp32, not from
+ * rounded copies).  The gradients of the hidden layer are rounded once to dtype, as operands of the
+ * products that follow.  dx must not overlap x or dy. */
+int prism_gated_ffn_backward(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
+                             const void* dy, void* dx, const prism_gated_grads* grads, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* The workspace of the forward (backward = 0) or backward (1) call: bounded, it does not grow with
+ * rows beyond some ten thousand. */
+int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_params* p, int backward, size_t* bytes);
+
 /* ---- fast path: a whole stack over a batch of frames ------------------------ */
 
 enum prism_block_kind { PRISM_BLOCK_MOE = 0, PRISM_BLOCK_DENSE = 1 };

@@ -19,8 +19,8 @@ from __future__ import annotations
 import ctypes as C
 
 from . import abi, configs, layout, synth
-from .abi import (AttnParams, DenseParams, DropoutParams, ExpertParams, NormParams, PrismError, ProjParams,
-                  RouterParams, check)
+from .abi import (AttnParams, DenseParams, DropoutParams, ExpertParams, GatedGrads, GatedParams, GatedWeights, NormParams,
+                  PrismError, ProjParams, RouterParams, check)
 from .layout import StackLayout, build_stack
 
 __all__ = ["Prism", "Stack", "AttnParams", "RouterParams", "ExpertParams", "ProjParams",
@@ -262,6 +262,55 @@ class Prism:
             self.h, C.byref(q), _ptr(x), _ptr(residual) if residual is not None else None,
             _flat(rng, "rng", (2,), torch.int64, x.device), _ptr(y), self._stream(stream)))
         return y
+
+    def _gated(self, x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
+        """(params, weights, rows, dim, hidden) of a gated feed-forward call."""
+        self._on_device(x, "x")
+        rows, dim, xs = _rows(x, "x")
+        hidden, dt, dev = w_gate.shape[0], x.dtype, x.device
+        if activation not in abi.ACTIVATIONS:
+            raise ValueError(f"activation {activation!r}: one of {', '.join(abi.ACTIVATIONS)}")
+        w = GatedWeights(_flat(w_gate, "w_gate", (hidden, dim), dt, dev), _flat(b_gate, "b_gate", (hidden,), dt, dev),
+                         _flat(w_up, "w_up", (hidden, dim), dt, dev), _flat(b_up, "b_up", (hidden,), dt, dev),
+                         _flat(w_down, "w_down", (dim, hidden), dt, dev), _flat(b_down, "b_down", (dim,), dt, dev))
+        p = GatedParams(rows=rows, x_stride=xs, dim=dim, hidden=hidden, dtype=_dtype(x, "x"),
+                        activation=abi.ACTIVATIONS.index(activation))
+        return p, w, rows, dim, hidden
+
+    def _gated_workspace(self, p, backward: int, workspace, device, stream):
+        need = C.c_size_t()
+        check(self.lib, self.lib.prism_gated_ffn_workspace(self.h, C.byref(p), backward, C.byref(need)))
+        return _workspace(workspace, need.value, device, stream)
+
+    def gated_ffn(self, x, w_gate, w_up, w_down, y, b_gate=None, b_up=None, b_down=None, residual=None,
+                  activation: str = "gelu", workspace=None, stream=None):
+        """prism_gated_ffn: y = w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down + residual, fp16 or
+        bf16; activation "gelu" (tanh form), "silu" or "relu"."""
+        p, w, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
+        p.y_stride = _rows(y, "y", (x, rows, dim))[2]
+        if residual is not None:
+            p.residual_stride = _rows(residual, "residual", (x, rows, dim))[2]
+        keep, ws, ws_bytes = self._gated_workspace(p, 0, workspace, x.device, stream)
+        check(self.lib, self.lib.prism_gated_ffn(self.h, C.byref(p), C.byref(w), _ptr(x),
+                                                 _ptr(residual) if residual is not None else None, _ptr(y), ws, ws_bytes,
+                                                 self._stream(stream)))
+        return y
+
+    def gated_ffn_backward(self, x, w_gate, w_up, w_down, dy, dx, dw_gate=None, dw_up=None, dw_down=None, b_gate=None,
+                           b_up=None, db_gate=None, db_up=None, db_down=None, activation: str = "gelu", workspace=None,
+                           stream=None):
+        """prism_gated_ffn_backward: dx and the parameters' gradients that are given (overwritten), from x, the
+        weights and dy; the forward pass has nothing to keep.  The residual's gradient is dy itself."""
+        p, w, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, None, activation)
+        like, dt, dev = (x, rows, dim), x.dtype, x.device
+        p.dy_stride, p.dx_stride = _rows(dy, "dy", like)[2], _rows(dx, "dx", like)[2]
+        d = GatedGrads(_flat(dw_gate, "dw_gate", (hidden, dim), dt, dev), _flat(db_gate, "db_gate", (hidden,), dt, dev),
+                       _flat(dw_up, "dw_up", (hidden, dim), dt, dev), _flat(db_up, "db_up", (hidden,), dt, dev),
+                       _flat(dw_down, "dw_down", (dim, hidden), dt, dev), _flat(db_down, "db_down", (dim,), dt, dev))
+        keep, ws, ws_bytes = self._gated_workspace(p, 1, workspace, dev, stream)
+        check(self.lib, self.lib.prism_gated_ffn_backward(self.h, C.byref(p), C.byref(w), _ptr(x), _ptr(dy), _ptr(dx),
+                                                          C.byref(d), ws, ws_bytes, self._stream(stream)))
+        return dx
 
     def status(self, stream=None):
         """prism_ctx_status: raises PrismError if a per-pass kernel's bounded wait gave up."""

@@ -72,6 +72,19 @@ class DropoutParams(C.Structure):
         _fields("dim dtype threshold")
 
 
+class GatedParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in "rows x_stride residual_stride y_stride dy_stride dx_stride".split()] + \
+        _fields("dim hidden dtype activation")
+
+
+class GatedWeights(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in "w_gate b_gate w_up b_up w_down b_down".split()]
+
+
+class GatedGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in "dw_gate db_gate dw_up db_up dw_down db_down".split()]
+
+
 def stack_desc(L: StackLayout):
     """(StackDesc, keep-alive block array) for a StackLayout."""
     arr = (BlockDesc * max(1, len(L.blocks)))()
@@ -99,13 +112,16 @@ EXPORTS = ("prism_create", "prism_destroy", "prism_last_error_string", "prism_ab
            "prism_expert_all_static", "prism_stack_inject_stall", "prism_stack_infer",
            "prism_stack_submit", "prism_stack_wait", "prism_moe_block", "prism_stack_infer_gpu",
            "prism_codec_pass", "prism_ctx_status", "prism_layer_norm", "prism_layer_norm_backward",
-           "prism_layer_norm_backward_workspace", "prism_dropout_add")
+           "prism_layer_norm_backward_workspace", "prism_dropout_add", "prism_gated_ffn",
+           "prism_gated_ffn_backward", "prism_gated_ffn_workspace")
 # prism_codec_kind order = the shaders of oracle.CODEC_KINDS
 CODEC_KINDS = ("conv3x3_coopvec_9ch", "strided_conv_coopvec_32ch", "strided_conv_split_64ch",
                "strided_conv_split_128ch", "dec3_fused", "dec2_fused", "dec1_fused",
                "pw_conv_coopvec_32to12", "pixelshuffle_sigmoid")
 # prism_dtype
 DTYPES = ("float16", "bfloat16", "float32")
+# prism_activation
+ACTIVATIONS = ("gelu", "silu", "relu")
 STATIC_MAX_TOKENS = 65536  # PRISM_STATIC_MAX_TOKENS
 # prism_stack_option
 OPT_PAIR_ATTENTION = 1
@@ -160,6 +176,10 @@ def load(path: os.PathLike | None = None) -> C.CDLL:
         "prism_layer_norm_backward": (i32, [vp, C.POINTER(NormParams)] + [vp] * 10 + [sz, vp]),
         "prism_layer_norm_backward_workspace": (i32, [vp, C.POINTER(NormParams), C.POINTER(sz)]),
         "prism_dropout_add": (i32, [vp, C.POINTER(DropoutParams), vp, vp, vp, vp, vp]),
+        "prism_gated_ffn": (i32, [vp, C.POINTER(GatedParams), C.POINTER(GatedWeights), vp, vp, vp, vp, sz, vp]),
+        "prism_gated_ffn_backward": (i32, [vp, C.POINTER(GatedParams), C.POINTER(GatedWeights), vp, vp, vp,
+                                           C.POINTER(GatedGrads), vp, sz, vp]),
+        "prism_gated_ffn_workspace": (i32, [vp, C.POINTER(GatedParams), i32, C.POINTER(sz)]),
         "prism_stack_profile_read": (i32, [vp, C.POINTER(C.c_double), C.POINTER(C.c_int64), i32]),
     }
     for name, (res, args) in sig.items():

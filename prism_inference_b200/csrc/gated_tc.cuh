@@ -1,0 +1,122 @@
+// gated_tc.cuh - CTA-pair (cta_group::2) building blocks of the gated feed-forward kernels: TMA loads
+// that complete on the leader's barrier, 256-row tcgen05 MMAs over both CTAs' shared memory and TMEM,
+// operand descriptors for both majors, and the gate's activations.
+#pragma once
+#include "train_util.cuh"
+
+namespace prism {
+
+enum GateAct : int { kActGelu = PRISM_ACT_GELU, kActSilu = PRISM_ACT_SILU, kActRelu = PRISM_ACT_RELU };
+
+// ---- pair TMA / MMA ------------------------------------------------------------------------
+// Loads into this CTA's shared memory; the bytes complete on an mbarrier of the pair's leader
+// (`bar` is a shared::cluster address).  No multicast.
+PRISM_DEV void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+PRISM_DEV void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+PRISM_DEV void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
+                 "r"(c0), "r"(c1)
+                 : "memory");
+}
+// fp32 box added to global memory in L2
+PRISM_DEV void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                 "r"(src), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+PRISM_DEV void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {  // one warp of each CTA
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+PRISM_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D (+)= A x B^T over the pair: rows 0..127 of A and of D in the leader, 128..255 in its peer; the
+// first half of B's N rows from the leader's shared memory, the second from the peer's.  Issued by one
+// elected lane of the leader's converged MMA warp.
+PRISM_DEV void mma_pair_ss_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrives on the barrier at this offset in both CTAs once every MMA issued before has completed
+PRISM_DEV void mma_commit_pair_w(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t.reg .b16 m;\n\t"
+        "mov.b16 m, 3;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+
+// Instruction descriptor, kind::f16, D fp32: formats (0 = fp16, 1 = bf16), majors (1 = MN), N, M.
+PRISM_DEV uint32_t idesc_pair(int M, int N, int bf16, int a_mn, int b_mn) {
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// MN-major operand in 128-byte swizzle: groups of 64 MN values, each [k][64] with 128 bytes a k row (8
+// rows = 1024 bytes, the stride field), `group_bytes` from one group of 64 to the next (the leading
+// field).  16 k further is 2048 bytes on.
+PRISM_DEV uint64_t sdesc_mn(uint32_t saddr, uint32_t group_bytes) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(group_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)SW128 << 61);
+}
+
+// ---- the gate ----------------------------------------------------------------------------------
+// 1 / (1 + 2^-t): both hardware approximations are good to about 2^-22, far under the 16-bit rounding
+// that follows (tanh.approx's 2^-11 would double the error of an fp16 result).
+PRISM_DEV float sigmoid_exp2(float t) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(-t)));
+    return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGelu2c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+// act(g); gelu as the framework's tanh form, written g sigmoid(2 sqrt(2/pi) (g + 0.044715 g^3))
+template <int ACT>
+PRISM_DEV float gate(float g) {
+    if (ACT == kActRelu) return g <= 0.0f ? 0.0f : g;  // NaN stays
+    if (ACT == kActSilu) return g * sigmoid_exp2(kLog2e * g);
+    const float z = g * fmaf(kGelu2c * kGeluA * kLog2e, g * g, kGelu2c * kLog2e);
+    return g * sigmoid_exp2(z);
+}
+// act(g) and act'(g)
+template <int ACT>
+PRISM_DEV void gate_grad(float g, float& a, float& d) {
+    if (ACT == kActRelu) {
+        a = g <= 0.0f ? 0.0f : g;
+        d = g > 0.0f ? 1.0f : 0.0f;
+        return;
+    }
+    if (ACT == kActSilu) {
+        const float s = sigmoid_exp2(kLog2e * g);
+        a = g * s;
+        d = fmaf(a, 1.0f - s, s);
+        return;
+    }
+    const float g2 = g * g;
+    const float s = sigmoid_exp2(g * fmaf(kGelu2c * kGeluA * kLog2e, g2, kGelu2c * kLog2e));
+    a = g * s;
+    d = fmaf(a * (1.0f - s), fmaf(3.0f * kGelu2c * kGeluA, g2, kGelu2c), s);
+}
+
+}  // namespace prism

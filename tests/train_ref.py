@@ -131,3 +131,69 @@ def act(g, kind):
     c, a = math.sqrt(2 / math.pi), 0.044715
     s = torch.sigmoid(2 * c * (g + a * g ** 3))
     return g * s, s + g * s * (1 - s) * 2 * c * (1 + 3 * a * g * g)
+
+
+# The kernels' sigmoid comes from two hardware approximations of about 2^-22 each; 2^-18 of the values
+# involved covers them and the roundings between.
+APPROX = 2.0 ** -18
+
+
+def _rounded(v, t, dtype):
+    """Error of v after one more rounding to `dtype`."""
+    return t + u(dtype) * (v.abs() + t) + TINY[dtype]
+
+
+def _hidden(x, wg, wu, bg, bu, kind):
+    """g, u, their error, act(g), act'(g) and the latter's error.  A product of n terms in the tensor cores'
+    fp32 accumulators, which need not round to nearest, is off by at most 2 n U32 of the magnitudes' sum."""
+    n = 2 * (x.shape[1] + 2) * U32
+    g, v = x @ wg.T + bg, x @ wu.T + bu
+    t_g, t_u = n * (x.abs() @ wg.abs().T + bg.abs()), n * (x.abs() @ wu.abs().T + bu.abs())
+    a, d = act(g, kind)
+    t_a = 1.2 * t_g + APPROX * a.abs()  # |act'| <= 1.13
+    # |act''| <= 0.8 (gelu), 0.5 (silu); relu's derivative jumps at 0, where g's error decides it
+    t_d = (g.abs() <= t_g).double() if kind == "relu" else t_g + APPROX * (1 + a.abs())
+    return g, v, t_u, a, t_a, d, t_d
+
+
+def gated(x, w, b, residual, kind, dtype):
+    """(y, tolerance).  w = (gate, up, down), b = (gate, up, down), None = zeros."""
+    x, (wg, wu, wd) = x.double(), (v.double() for v in w)
+    bg, bu, bd = (torch.zeros(n, dtype=torch.float64, device=x.device) if v is None else v.double()
+                  for v, n in zip(b, (wg.shape[0], wg.shape[0], wd.shape[0])))
+    g, v, t_u, a, t_a, _, _ = _hidden(x, wg, wu, bg, bu, kind)
+    h = a * v
+    t_h = _rounded(h, t_a * (v.abs() + t_u) + a.abs() * t_u + 2 * U32 * h.abs(), dtype)
+    y = h @ wd.T + bd
+    t = t_h @ wd.abs().T + 2 * (h.shape[1] + 2) * U32 * ((h.abs() + t_h) @ wd.abs().T + bd.abs())
+    if residual is not None:
+        y = y + residual.double()
+        t = t + 2 * U32 * (residual.double().abs() + y.abs())
+    return y, t
+
+
+def gated_back(x, w, b, dy, kind, dtype):
+    """{name: (gradient, tolerance)}"""
+    x, dy, (wg, wu, wd) = x.double(), dy.double(), (v.double() for v in w)
+    R, H = x.shape[0], wg.shape[0]
+    bg, bu = (torch.zeros(H, dtype=torch.float64, device=x.device) if v is None else v.double() for v in b[:2])
+    g, v, t_u, a, t_a, d, t_d = _hidden(x, wg, wu, bg, bu, kind)
+    dh = dy @ wd
+    t_dh = 2 * (dy.shape[1] + 2) * U32 * (dy.abs() @ wd.abs())
+    h, du, dg = a * v, dh * a, dh * v * d
+    dha, va, aa, da = dh.abs() + t_dh, v.abs() + t_u, a.abs() + t_a, d.abs() + t_d
+    t_h = _rounded(h, t_a * va + a.abs() * t_u + 2 * U32 * h.abs(), dtype)
+    t_du = _rounded(du, t_dh * aa + dh.abs() * t_a + 2 * U32 * du.abs(), dtype)
+    t_dg = _rounded(dg, t_dh * va * da + dha * t_u * da + dha * va * t_d + 4 * U32 * dg.abs(), dtype)
+    kx, kr = 2 * (2 * H + 2) * U32, 2 * (R + 2) * U32
+
+    def rows(p, t_p, q):  # p^T q over the rows
+        return p.T @ q, t_p.T @ q.abs() + kr * ((p.abs() + t_p).T @ q.abs())
+    one = torch.ones((R, 1), dtype=torch.float64, device=x.device)
+    dwd, t_dwd = rows(h, t_h, dy)
+    out = {"dx": (dg @ wg + du @ wu, t_dg @ wg.abs() + t_du @ wu.abs() + kx * ((dg.abs() + t_dg) @ wg.abs() + (du.abs() + t_du) @ wu.abs())),
+           "dw_gate": rows(dg, t_dg, x), "dw_up": rows(du, t_du, x), "dw_down": (dwd.T, t_dwd.T)}
+    for n, p, t in (("db_gate", dg, t_dg), ("db_up", du, t_du), ("db_down", dy, torch.zeros_like(dy))):
+        s, ts = rows(p, t, one)
+        out[n] = (s[:, 0], ts[:, 0])
+    return out
