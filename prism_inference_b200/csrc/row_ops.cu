@@ -9,40 +9,140 @@ namespace prism {
 namespace {
 
 // ---- rows in registers ---------------------------------------------------------------------
-// A team of TEAM threads holds one row: thread t owns the NV groups of VEC consecutive columns
-// that start at (j * TEAM + t) * VEC.  VEC values are one 16-byte access where base and stride
-// allow it (VEC > 1), single values otherwise.  A row's last, partial group goes by single values.
-template <typename T, int VEC, int TEAM, int NV>
-struct Row {
-    static constexpr int kN = VEC * NV;
-    PRISM_DEV static int col(int t, int j) { return (j * TEAM + t) * VEC; }
+// A team of TEAM threads holds one row: thread t owns the NV groups of VEC consecutive columns that
+// start at (j * TEAM + t) * VEC, VEC values = 16 bytes.  16 values a thread: with a whole warp on a
+// 256-wide row the butterflies and the loop cost more instructions than the row's arithmetic (199
+// against 94 us for 522,240 rows of fp16).
+template <typename T>
+struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    union {
+        uint4 q;
+        T v[N];
+    };
+    PRISM_DEV Pack() {}
+};
+template <typename T>
+struct RowTensor {
+    T* p;
+    int64_t stride;
 };
 
-template <typename T, int VEC>
-struct alignas(VEC * sizeof(T)) Pack {
-    T v[VEC];
-};
+// first column of group j of thread t
+template <typename T, int TEAM>
+PRISM_DEV int col_of(int t, int j) { return (j * TEAM + t) * Pack<T>::N; }
 
-template <typename T, int VEC>
-PRISM_DEV Pack<T, VEC> load_pack(const T* row, int c, int dim) {
-    Pack<T, VEC> p;
-    if (c + VEC <= dim) {
-        p = *reinterpret_cast<const Pack<T, VEC>*>(row + c);
+// FAST kernels know that every row of every tensor starts on a 16-byte boundary and that dim is a
+// multiple of a group.  The others take rows at any multiple of the type's size, m bytes past a
+// 16-byte boundary: memory is still read and written in aligned 16-byte chunks, and a thread's group is
+// cut out of its own chunk and the next thread's (a shuffle).  (Single-value accesses instead: 310
+// against 137 us for 65,536 x 1001 fp16 forward.)
+PRISM_DEV uint4 shift_down(const uint4& a, const uint4& b, uint32_t m) {  // bytes m .. m + 15 of a, b
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (m & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (m & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const uint32_t bits = (m & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                      __funnelshift_r(w[3], w[4], bits));
+}
+// the chunk at `at`, of which only [lo, hi) is the tensor's memory
+template <typename T>
+PRISM_DEV uint4 load_chunk(const char* at, const char* lo, const char* hi) {
+    Pack<T> p;
+    if (at >= lo && at + 16 <= hi) {
+        p.q = *reinterpret_cast<const uint4*>(at);
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) p.v[e] = c + e < dim ? row[c + e] : from_f32<T>(0.0f);
+        for (int e = 0; e < Pack<T>::N; ++e) {
+            const char* v = at + e * sizeof(T);
+            p.v[e] = v >= lo && v < hi ? *reinterpret_cast<const T*>(v) : from_f32<T>(0.0f);
+        }
+    }
+    return p.q;
+}
+PRISM_DEV uint4 shfl_next(const uint4& v, int delta) {  // from the lane `delta` further
+    return make_uint4(__shfl_sync(0xffffffffu, v.x, (threadIdx.x + delta) & 31), __shfl_sync(0xffffffffu, v.y, (threadIdx.x + delta) & 31),
+                      __shfl_sync(0xffffffffu, v.z, (threadIdx.x + delta) & 31), __shfl_sync(0xffffffffu, v.w, (threadIdx.x + delta) & 31));
+}
+
+// Group j of this thread's row as loaded (`settle` turns it into values, so that loads can be in flight
+// while the row before is worked on).
+template <bool FAST>
+struct Raw {
+    uint4 own, next;
+};
+template <>
+struct Raw<true> {
+    uint4 own;
+};
+template <bool FAST, typename T, int TEAM>
+PRISM_DEV Raw<FAST> load_group(const RowTensor<const T>& x, int64_t row, int64_t rows, int dim, int t, int j) {
+    constexpr int VEC = Pack<T>::N, kSeg = TEAM < 32 ? TEAM : 32;  // threads whose chunks follow one another in a warp
+    const int c = col_of<T, TEAM>(t, j);
+    Raw<FAST> p;
+    p.own = make_uint4(0, 0, 0, 0);
+    const bool in = row < rows;
+    const T* src = x.p + (in ? row : 0) * x.stride + c;
+    if constexpr (FAST) {
+        if (in && c < dim) p.own = *reinterpret_cast<const uint4*>(src);
+    } else {
+        const char *lo = reinterpret_cast<const char*>(x.p), *hi = reinterpret_cast<const char*>(x.p + (rows - 1) * x.stride + dim);
+        const uint32_t m = (uint32_t)(uintptr_t)src & 15u;
+        const char* at = reinterpret_cast<const char*>(src) - m;
+        // this chunk holds columns from c - m / size on: wanted by this thread and the one before
+        if (in && c < dim + VEC) p.own = load_chunk<T>(at, lo, hi);
+        p.next = make_uint4(0, 0, 0, 0);
+        if (t % kSeg == kSeg - 1 && in && m && c < dim) p.next = load_chunk<T>(at + 16, lo, hi);
     }
     return p;
 }
-template <typename T, int VEC>
-PRISM_DEV void store_pack(T* row, int c, int dim, const Pack<T, VEC>& p) {
-    if (c + VEC <= dim) {
-        *reinterpret_cast<Pack<T, VEC>*>(row + c) = p;
-    } else {
+// its values, zeros outside [0, rows) x [0, dim).  Whole warps (the shuffles).
+template <bool FAST, typename T, int TEAM>
+PRISM_DEV Pack<T> settle(const Raw<FAST>& raw, const RowTensor<const T>& x, int64_t row, int64_t rows, int dim, int t, int j) {
+    constexpr int VEC = Pack<T>::N, kSeg = TEAM < 32 ? TEAM : 32;
+    Pack<T> p;
+    p.q = raw.own;
+    if constexpr (!FAST) {
+        const int c = col_of<T, TEAM>(t, j);
+        const bool in = row < rows;
+        const uint32_t m = (uint32_t)(uintptr_t)(x.p + (in ? row : 0) * x.stride + c) & 15u;
+        uint4 next = shfl_next(p.q, 1);
+        if (t % kSeg == kSeg - 1) next = raw.next;
+        p.q = shift_down(p.q, next, m);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-            if (c + e < dim) row[c + e] = p.v[e];
+            if (!in || c + e >= dim) p.v[e] = from_f32<T>(0.0f);
     }
+    return p;
+}
+template <bool FAST, typename T, int TEAM>
+PRISM_DEV void store_group(const RowTensor<T>& y, int64_t row, int64_t rows, int dim, int t, int j, const Pack<T>& p) {
+    constexpr int VEC = Pack<T>::N, kSeg = TEAM < 32 ? TEAM : 32;
+    const int c = col_of<T, TEAM>(t, j);
+    const bool in = row < rows;
+    T* dst = y.p + (in ? row : 0) * y.stride + c;
+    if (FAST) {
+        if (in && c < dim) *reinterpret_cast<uint4*>(dst) = p.q;
+        return;
+    }
+    // The aligned chunk at dst - m: the last m bytes of the group before and the first 16 - m of this
+    // one.  Chunks that are not wholly of this row, or whose other group another warp has, go value by
+    // value.
+    const uint32_t m = (uint32_t)(uintptr_t)dst & 15u;
+    const int n0 = (int)((16 - m) / sizeof(T)), s = t % kSeg;
+    const uint4 before = shfl_next(p.q, -1);
+    const bool mine = (m == 0 || s > 0) && c + n0 <= dim, later = s < kSeg - 1 && c + VEC + n0 <= dim;
+    if (!in) return;
+    if (mine) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(dst) - m) = m ? shift_down(before, p.q, 16 - m) : p.q;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        if (c + e < dim && !(e < n0 ? mine : later)) dst[e] = p.v[e];
 }
 // a parameter vector's value: fp32, or the rows' type T
 template <typename T>
@@ -50,25 +150,50 @@ PRISM_DEV float param_at(const void* w, int f32, int c) {
     return f32 ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
 }
 
-// Sums of two values over a team.  Teams of up to a warp: butterfly, every lane gets the same bits.
-// Teams of a whole CTA: butterfly, then the warps' sums in order from shared memory.
-template <int TEAM>
-PRISM_DEV void team_sum2(float& a, float& b, float2* red) {
+// columns c .. c + VEC - 1 of a parameter vector, `none` where there is none
+template <typename T>
+PRISM_DEV void load_params(const void* w, int f32, int c, int dim, float none, float* out) {
+    constexpr int VEC = Pack<T>::N;
+    if (w && c + VEC <= dim && (uintptr_t)w % 16 == 0) {
+        if (f32) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + c + e);
+                out[e] = v.x, out[e + 1] = v.y, out[e + 2] = v.z, out[e + 3] = v.w;
+            }
+        } else {
+            Pack<T> p;
+            p.q = *reinterpret_cast<const uint4*>(static_cast<const T*>(w) + c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = to_f32(p.v[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out[e] = w && c + e < dim ? param_at<T>(w, f32, c + e) : none;
+    }
+}
+
+// Sums over a team.  Teams of up to a warp: butterfly, every lane gets the same bits.  Larger teams:
+// butterfly, then the warps' sums in order from shared memory, between barriers of the team's own.
+template <int TEAM, int N>
+PRISM_DEV void team_sum(float (&a)[N], float2* red) {
     constexpr int kW = TEAM < 32 ? TEAM : 32;
 #pragma unroll
     for (int o = kW / 2; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
     }
     if (TEAM > 32) {
-        __syncthreads();  // the sums of the call before have been read
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a, b);
-        __syncthreads();
-        a = b = 0.0f;
+        const int first = (threadIdx.x / TEAM) * (TEAM / 32), bar = 1 + threadIdx.x / TEAM;
+        named_bar_sync(bar, TEAM);  // the sums of the call before have been read
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a[0], a[N - 1]);
+        named_bar_sync(bar, TEAM);
+        a[0] = a[N - 1] = 0.0f;
 #pragma unroll
         for (int w = 0; w < TEAM / 32; ++w) {
-            a += red[w].x;
-            b += red[w].y;
+            const float2 v = red[first + w];
+            a[0] += v.x;
+            if (N > 1) a[N - 1] += v.y;
         }
     }
 }
@@ -90,179 +215,190 @@ struct NormBackArgs {
     int dim, param_f32;
 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+// the first row of this warp, and this lane's row
+template <int TEAM>
+PRISM_DEV int64_t warp_row() {
+    constexpr int kTeams = kThreads / TEAM;
+    return (int64_t)blockIdx.x * kTeams + (TEAM < 32 ? (threadIdx.x / 32) * (32 / TEAM) : threadIdx.x / TEAM);
+}
 
 // y = (x - mean) rstd w + b.  One pass over memory: the row stays in registers between the mean,
 // the centred second moment and the output.  Memory-bound: 2 R D s bytes.  The next row's loads
 // are issued before this row's sums, so each team keeps two rows in flight.
-template <typename T, int VEC, int TEAM, int NV>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
-    using R = Row<T, VEC, TEAM, NV>;
-    __shared__ float2 red[kThreads / 32];
-    constexpr int kTeams = kThreads / TEAM;
-    constexpr bool kHold = R::kN <= 16;  // weight and bias stay in registers across rows
+template <bool FAST, typename T, int TEAM, int NV>
+__global__ void __launch_bounds__(kThreads, FAST && NV * Pack<T>::N <= 16 ? 3 : 1) norm_kernel(const NormArgs a) {
+    constexpr int VEC = Pack<T>::N, kN = VEC * NV, kTeams = kThreads / TEAM;
+    constexpr bool kHold = kN <= 16;  // weight and bias stay in registers across rows
+    __shared__ float2 red[kWarps];
     const int t = threadIdx.x % TEAM;
     const int64_t step = (int64_t)gridDim.x * kTeams;
-    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / TEAM;
-    const T* x = static_cast<const T*>(a.x);
-    T* y = static_cast<T*>(a.y);
+    const RowTensor<const T> x{static_cast<const T*>(a.x), a.xs};
+    const RowTensor<T> y{static_cast<T*>(a.y), a.ys};
     const float inv = 1.0f / (float)a.dim;
-    float w[kHold ? R::kN : 1], b[kHold ? R::kN : 1];
+    Raw<FAST> nxt[NV];
+    // every lane of a warp walks the same number of rows (the shuffles need the whole warp); teams
+    // past the last row work on zeros and store nothing
+    int64_t row0 = warp_row<TEAM>();
+    const int team = TEAM < 32 ? (threadIdx.x & 31) / TEAM : 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) nxt[j] = load_group<FAST, T, TEAM>(x, row0 + team, a.rows, a.dim, t, j);
+    float w[kHold ? kN : VEC], b[kHold ? kN : VEC];
     if (kHold) {
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
-            const int c = R::col(t, i / VEC) + i % VEC;
-            w[i] = a.weight && c < a.dim ? param_at<T>(a.weight, a.param_f32, c) : 1.0f;
-            b[i] = a.bias && c < a.dim ? param_at<T>(a.bias, a.param_f32, c) : 0.0f;
+        for (int j = 0; j < NV; ++j) {
+            load_params<T>(a.weight, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 1.0f, w + j * VEC);
+            load_params<T>(a.bias, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 0.0f, b + j * VEC);
         }
     }
-    Pack<T, VEC> cur[NV], nxt[NV];
-    // every thread of a warp runs the same number of rows (the shuffles need the whole warp);
-    // teams past the last row work on zeros and store nothing
-    auto load = [&](Pack<T, VEC>(&p)[NV], int64_t r) {
-        const T* src = x + (r < a.rows ? r : 0) * a.xs;
-        const int lim = r < a.rows ? a.dim : 0;
+    for (; row0 < a.rows; row0 += step) {
+        Pack<T> cur[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) p[j] = load_pack<T, VEC>(src, R::col(t, j), lim);
-    };
-    const int64_t first = (int64_t)blockIdx.x * kTeams + (TEAM < 32 ? (threadIdx.x / 32) * (32 / TEAM) : threadIdx.x / TEAM);
-    load(cur, row);
-    for (int64_t lead = first; lead < a.rows; lead += step, row += step) {
-        if (lead + step < a.rows) load(nxt, row + step);
-        float v[R::kN], s0 = 0.0f, s1 = 0.0f;
+        for (int j = 0; j < NV; ++j) cur[j] = settle<FAST, T, TEAM>(nxt[j], x, row0 + team, a.rows, a.dim, t, j);
+        if (row0 + step < a.rows) {
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
+            for (int j = 0; j < NV; ++j) nxt[j] = load_group<FAST, T, TEAM>(x, row0 + step + team, a.rows, a.dim, t, j);
+        }
+        float v[kN], s[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
             v[i] = to_f32(cur[i / VEC].v[i % VEC]);
-            s0 += v[i];
+            s[0] += v[i];
         }
-        team_sum2<TEAM>(s0, s1, red);
-        const float mean = s0 * inv;
-        float q = 0.0f;
+        team_sum<TEAM>(s, red);
+        const float mean = s[0] * inv;
+        s[0] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
+        for (int i = 0; i < kN; ++i) {
             v[i] -= mean;
-            if (R::col(t, i / VEC) + i % VEC < a.dim) q = fmaf(v[i], v[i], q);
+            const int c = (i / VEC * TEAM + t) * VEC + (FAST ? 0 : i % VEC);
+            if (c < a.dim) s[0] = fmaf(v[i], v[i], s[0]);
         }
-        s1 = 0.0f;
-        team_sum2<TEAM>(q, s1, red);
-        const float rstd = rsqrtf(fmaf(q, inv, a.eps));
-        if (row < a.rows) {
-            T* dst = y + row * a.ys;
+        team_sum<TEAM>(s, red);
+        const float rstd = rsqrtf(fmaf(s[0], inv, a.eps));
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = R::col(t, j);
-                Pack<T, VEC> o;
+        for (int j = 0; j < NV; ++j) {
+            if (!kHold) {
+                load_params<T>(a.weight, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 1.0f, w);
+                load_params<T>(a.bias, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 0.0f, b);
+            }
+            Pack<T> o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = j * VEC + e;
-                    float wi, bi;
-                    if (kHold) {
-                        wi = w[kHold ? i : 0];
-                        bi = b[kHold ? i : 0];
-                    } else {
-                        wi = a.weight && c + e < a.dim ? param_at<T>(a.weight, a.param_f32, c + e) : 1.0f;
-                        bi = a.bias && c + e < a.dim ? param_at<T>(a.bias, a.param_f32, c + e) : 0.0f;
-                    }
-                    o.v[e] = from_f32<T>(fmaf(v[i] * rstd, wi, bi));
-                }
-                store_pack<T, VEC>(dst, c, a.dim, o);
+            for (int e = 0; e < VEC; ++e) {
+                const int i = j * VEC + e, k = kHold ? i : e;
+                o.v[e] = from_f32<T>(fmaf(v[i] * rstd, w[k], b[k]));
             }
-            if (t == 0) {
-                if (a.mean) a.mean[row] = mean;
-                if (a.rstd) a.rstd[row] = rstd;
-            }
+            store_group<FAST, T, TEAM>(y, row0 + team, a.rows, a.dim, t, j, o);
         }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) cur[j] = nxt[j];
+        if (t == 0 && row0 + team < a.rows) {
+            if (a.mean) a.mean[row0 + team] = mean;
+            if (a.rstd) a.rstd[row0 + team] = rstd;
+        }
     }
 }
 
 // With xh = (x - mean) rstd and g = dy w:
 //   dx = rstd (g - mean_c(g) - xh mean_c(g xh)) [+ add],  dweight = sum_r dy xh,  dbias = sum_r dy.
 // One pass over x and dy: each thread keeps its columns' dweight and dbias sums over all the rows
-// its team walks, the CTA's teams are added in order, and norm_fold_kernel adds the CTAs' partial
+// its team walks, the CTA's warps are added in order, and norm_fold_kernel adds the CTAs' partial
 // sums in order (no atomics: the same inputs give the same bits).
-template <typename T, int VEC, int TEAM, int NV>
-__global__ void __launch_bounds__(kThreads) norm_back_kernel(const NormBackArgs a) {
-    using R = Row<T, VEC, TEAM, NV>;
-    extern __shared__ float fold[];  // [2][dim], teams smaller than the CTA
-    __shared__ float2 red[kThreads / 32];
-    constexpr int kTeams = kThreads / TEAM;
-    constexpr bool kHold = R::kN <= 16;
-    const int t = threadIdx.x % TEAM;
+// the registers that two CTAs an SM leave each thread hold 16 16-bit values' sums and loads, no more
+template <bool FAST, typename T, int NV>
+__host__ __device__ constexpr int back_ctas_per_sm() {
+    return FAST && sizeof(T) == 2 && NV * Pack<T>::N <= 16 ? 2 : 1;
+}
+template <bool FAST, typename T, int TEAM, int NV>
+__global__ void __launch_bounds__(kThreads, back_ctas_per_sm<FAST, T, NV>()) norm_back_kernel(const NormBackArgs a) {
+    constexpr int VEC = Pack<T>::N, kN = VEC * NV, kTeams = kThreads / TEAM;
+    constexpr bool kHold = kN <= 16;
+    constexpr int kParts = TEAM < 32 ? kWarps : kTeams;  // sums of whole columns in a CTA: warps or teams
+    extern __shared__ float fold[];  // [kParts][2][dim], teams smaller than the CTA
+    __shared__ float2 red[kWarps];
+    const int t = threadIdx.x % TEAM, team = TEAM < 32 ? (threadIdx.x & 31) / TEAM : 0;
     const int64_t step = (int64_t)gridDim.x * kTeams;
-    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / TEAM;
-    const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy), *add = static_cast<const T*>(a.add);
-    T* dx = static_cast<T*>(a.dx);
+    const RowTensor<const T> x{static_cast<const T*>(a.x), a.xs}, dy{static_cast<const T*>(a.dy), a.dys},
+        add{static_cast<const T*>(a.add), a.adds};
+    const RowTensor<T> dx{static_cast<T*>(a.dx), a.dxs};
     const float inv = 1.0f / (float)a.dim;
-    float w[kHold ? R::kN : 1];
-    if (kHold) {
+    float dw[kN], db[kN];
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
-            const int c = R::col(t, i / VEC) + i % VEC;
-            w[i] = a.weight && c < a.dim ? param_at<T>(a.weight, a.param_f32, c) : 1.0f;
-        }
-    }
-    float dw[R::kN], db[R::kN];
-#pragma unroll
-    for (int i = 0; i < R::kN; ++i) dw[i] = db[i] = 0.0f;
-    const int64_t first = (int64_t)blockIdx.x * kTeams + (TEAM < 32 ? (threadIdx.x / 32) * (32 / TEAM) : threadIdx.x / TEAM);
-    for (int64_t lead = first; lead < a.rows; lead += step, row += step) {
-        const bool in = row < a.rows;
-        const int64_t r = in ? row : 0;
-        const int lim = in ? a.dim : 0;
-        const float mean = in ? a.mean[r] : 0.0f, rstd = in ? a.rstd[r] : 0.0f;
-        Pack<T, VEC> px[NV], pg[NV];
+    for (int i = 0; i < kN; ++i) dw[i] = db[i] = 0.0f;
+    int64_t row0 = warp_row<TEAM>();
+    // the next row's loads are in flight during this row's sums and its store
+    Raw<FAST> nx[NV], ng[NV], na[NV];
+    float mean = 0.0f, rstd = 0.0f;
+    auto load = [&](int64_t r0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            px[j] = load_pack<T, VEC>(x + r * a.xs, R::col(t, j), lim);
-            pg[j] = load_pack<T, VEC>(dy + r * a.dys, R::col(t, j), lim);
+            nx[j] = load_group<FAST, T, TEAM>(x, r0 + team, a.rows, a.dim, t, j);
+            ng[j] = load_group<FAST, T, TEAM>(dy, r0 + team, a.rows, a.dim, t, j);
+            if (add.p) na[j] = load_group<FAST, T, TEAM>(add, r0 + team, a.rows, a.dim, t, j);
         }
-        float g[R::kN], xh[R::kN], s0 = 0.0f, s1 = 0.0f;
+        const bool in = r0 + team < a.rows;
+        mean = in ? a.mean[r0 + team] : 0.0f;
+        rstd = in ? a.rstd[r0 + team] : 0.0f;
+    };
+    load(row0);
+    float w[kHold ? kN : VEC];
+    if (kHold) {
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
-            const int c = R::col(t, i / VEC) + i % VEC;
-            const float d = to_f32(pg[i / VEC].v[i % VEC]);
-            // columns past the row hold zeros, whose xh is not zero: they take no part
-            xh[i] = c < lim ? (to_f32(px[i / VEC].v[i % VEC]) - mean) * rstd : 0.0f;
-            float wi;
-            if (kHold)
-                wi = w[kHold ? i : 0];
-            else
-                wi = a.weight && c < a.dim ? param_at<T>(a.weight, a.param_f32, c) : 1.0f;
-            g[i] = d * wi;
-            dw[i] = fmaf(d, xh[i], dw[i]);
+        for (int j = 0; j < NV; ++j) load_params<T>(a.weight, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 1.0f, w + j * VEC);
+    }
+    for (; row0 < a.rows; row0 += step) {
+        const float m = mean, r = rstd;
+        float s[2] = {0.0f, 0.0f};
+        // columns past the row hold zeros, whose xh is not zero: they take no part (as rows past the last)
+        const int lim = row0 + team < a.rows ? a.dim : 0;
+        Pack<T> px[NV], pg[NV], pa[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            px[j] = settle<FAST, T, TEAM>(nx[j], x, row0 + team, a.rows, a.dim, t, j);
+            pg[j] = settle<FAST, T, TEAM>(ng[j], dy, row0 + team, a.rows, a.dim, t, j);
+            if (add.p) pa[j] = settle<FAST, T, TEAM>(na[j], add, row0 + team, a.rows, a.dim, t, j);
+        }
+        if (row0 + step < a.rows) load(row0 + step);
+        // dy and x stay as loaded: g and xh are worked out again after the sums, which costs less than
+        // the registers to keep them
+        auto value = [&](int i, float& d, float& g, float& xh) {
+            const int c = (i / VEC * TEAM + t) * VEC + (FAST ? 0 : i % VEC);
+            d = to_f32(pg[i / VEC].v[i % VEC]);
+            xh = c < lim ? (to_f32(px[i / VEC].v[i % VEC]) - m) * r : 0.0f;
+            g = d * w[kHold ? i : i % VEC];
+        };
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if (!kHold && i % VEC == 0) load_params<T>(a.weight, a.param_f32, col_of<T, TEAM>(t, i / VEC), a.dim, 1.0f, w);
+            float d, g, xh;
+            value(i, d, g, xh);
+            dw[i] = fmaf(d, xh, dw[i]);
             db[i] += d;
-            s0 += g[i];
-            s1 = fmaf(g[i], xh[i], s1);
+            s[0] += g;
+            s[1] = fmaf(g, xh, s[1]);
         }
-        team_sum2<TEAM>(s0, s1, red);
-        const float m0 = s0 * inv, m1 = s1 * inv;
-        if (in) {
+        team_sum<TEAM>(s, red);
+        const float m0 = s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = R::col(t, j);
-                Pack<T, VEC> o, pa;
-                if (add) pa = load_pack<T, VEC>(add + r * a.adds, c, a.dim);
+        for (int j = 0; j < NV; ++j) {
+            if (!kHold) load_params<T>(a.weight, a.param_f32, col_of<T, TEAM>(t, j), a.dim, 1.0f, w);
+            Pack<T> o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = j * VEC + e;
-                    float d = rstd * (g[i] - m0 - xh[i] * m1);
-                    if (add) d += to_f32(pa.v[e]);
-                    o.v[e] = from_f32<T>(d);
-                }
-                store_pack<T, VEC>(dx + r * a.dxs, c, a.dim, o);
+            for (int e = 0; e < VEC; ++e) {
+                float d, g, xh;
+                value(j * VEC + e, d, g, xh);
+                d = r * (g - m0 - xh * m1);
+                if (add.p) d += to_f32(pa[j].v[e]);
+                o.v[e] = from_f32<T>(d);
             }
+            store_group<FAST, T, TEAM>(dx, row0 + team, a.rows, a.dim, t, j, o);
         }
     }
     if (!a.part) return;
     float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
     if (TEAM < kThreads) {
-        // a warp's teams by butterfly, then the warps one after the other
-        constexpr int kWarps = kThreads / 32;
-        if (TEAM < 32) {
+        if (TEAM < 32) {  // a warp's teams by butterfly
 #pragma unroll
-            for (int i = 0; i < R::kN; ++i) {
+            for (int i = 0; i < kN; ++i) {
 #pragma unroll
                 for (int o = TEAM; o < 32; o <<= 1) {
                     dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
@@ -270,24 +406,28 @@ __global__ void __launch_bounds__(kThreads) norm_back_kernel(const NormBackArgs 
                 }
             }
         }
-        for (int wp = 0; wp < kWarps; ++wp) {
-            if ((int)(threadIdx.x >> 5) == wp && (threadIdx.x & 31) < TEAM) {
+        float* mine = fold + (threadIdx.x / (TEAM < 32 ? 32 : TEAM)) * 2 * a.dim;
+        if (TEAM >= 32 || (threadIdx.x & 31) < TEAM) {
 #pragma unroll
-                for (int i = 0; i < R::kN; ++i) {
-                    const int c = R::col(t, i / VEC) + i % VEC;
-                    if (c < a.dim) {
-                        fold[c] = wp ? fold[c] + dw[i] : dw[i];
-                        fold[a.dim + c] = wp ? fold[a.dim + c] + db[i] : db[i];
-                    }
+            for (int i = 0; i < kN; ++i) {
+                const int c = (i / VEC * TEAM + t) * VEC + i % VEC;
+                if (c < a.dim) {
+                    mine[c] = dw[i];
+                    mine[a.dim + c] = db[i];
                 }
             }
-            __syncthreads();
         }
-        for (int c = threadIdx.x; c < 2 * a.dim; c += kThreads) out[c] = fold[c];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * a.dim; c += kThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) s += fold[k * 2 * a.dim + c];
+            out[c] = s;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < R::kN; ++i) {
-            const int c = R::col(t, i / VEC) + i % VEC;
+        for (int i = 0; i < kN; ++i) {
+            const int c = (i / VEC * TEAM + t) * VEC + i % VEC;
             if (c < a.dim) {
                 out[c] = dw[i];
                 out[a.dim + c] = db[i];
@@ -296,24 +436,24 @@ __global__ void __launch_bounds__(kThreads) norm_back_kernel(const NormBackArgs 
     }
 }
 
-// Adds the CTAs' partial sums: 32 columns a CTA, 8 threads a column over every 8th partial, then the 8
-// in order.
+// Adds the CTAs' partial sums: 32 columns a CTA, 32 threads a column over every 32nd partial, then the
+// 32 in order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(1024)
     norm_fold_kernel(const float* part, int n_part, int dim, void* dweight, void* dbias, int param_f32) {
-    __shared__ float red[8][33];
+    __shared__ float red[32][33];
     grid_dep_wait();
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;  // over [dweight | dbias]
     float s = 0.0f;
     if (c < 2 * dim)
-        for (int p = k; p < n_part; p += 8) s += part[(int64_t)p * 2 * dim + c];
+        for (int p = k; p < n_part; p += 32) s += part[(int64_t)p * 2 * dim + c];
     red[k][lane] = s;
     __syncthreads();
     if (k == 0 && c < 2 * dim) {
         s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += red[i][lane];
+        for (int i = 0; i < 32; ++i) s += red[i][lane];
         void* dst = c < dim ? dweight : dbias;
         const int i = c < dim ? c : c - dim;
         if (dst) {
@@ -364,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
     constexpr int UNR = 2, E = 16 / sizeof(T);
     for (int64_t b0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; b0 < blocks; b0 += UNR * stride) {
         if (VEC8) {
-            Pack<T, E> px[UNR][8 / E], pr[UNR][8 / E];
+            Pack<T> px[UNR][8 / E], pr[UNR][8 / E];
             int64_t yo[UNR];
             bool full[UNR];
 #pragma unroll
@@ -381,8 +521,8 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
                 yo[u] = r * a.ys + c;
 #pragma unroll
                 for (int q = 0; q < 8 / E; ++q) {
-                    px[u][q] = *reinterpret_cast<const Pack<T, E>*>(x + r * a.xs + c + q * E);
-                    if (res) pr[u][q] = *reinterpret_cast<const Pack<T, E>*>(res + r * a.rs + c + q * E);
+                    px[u][q].q = *reinterpret_cast<const uint4*>(x + r * a.xs + c + q * E);
+                    if (res) pr[u][q].q = *reinterpret_cast<const uint4*>(res + r * a.rs + c + q * E);
                 }
             }
 #pragma unroll
@@ -394,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
                 if (full[u]) {
 #pragma unroll
                     for (int q = 0; q < 8 / E; ++q) {
-                        Pack<T, E> o;
+                        Pack<T> o;
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
                             const int i = q * E + e;
@@ -402,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
                             const float v = h >= a.threshold ? to_f32(px[u][q].v[e]) * a.scale : 0.0f;
                             o.v[e] = from_f32<T>(res ? v + to_f32(pr[u][q].v[e]) : v);
                         }
-                        *reinterpret_cast<Pack<T, E>*>(y + yo[u] + q * E) = o;
+                        *reinterpret_cast<uint4*>(y + yo[u] + q * E) = o.q;
                     }
                 } else {  // the last block of a flat tensor (rows of a strided one are multiples of 8)
 #pragma unroll
@@ -452,31 +592,27 @@ int cuda_rc(cudaError_t e, const char* what) {
 }
 
 constexpr int kNormMaxDim = 16384;
-constexpr int kBackCtasPerSm = 2;
+constexpr int kBackCtasPerSm = 2;  // at most: sizes the workspace
 
-// What a row's threads hold, by type, alignment and width: f(T{}, VEC, TEAM, NV) as constants.
+// What a row's threads hold, by type and width: f(FAST, TEAM, NV) as constants.  16 values a thread up to
+// the width of a CTA's 256 threads (with a warp and 32 values on 1000-wide rows, backward: 208 against
+// 108 us for 65,536 rows of fp16, for want of warps), then more.
 template <typename T, typename F>
-int with_shape(bool vec, int dim, F&& f) {
-    constexpr int V = 16 / sizeof(T);
+int with_shape(bool fast, int dim, F&& f) {
+    constexpr int V = Pack<T>::N, NV = 16 / V;
     using std::integral_constant;
-#define SHAPE(VEC, TEAM, NV) \
-    return f(integral_constant<int, VEC>{}, integral_constant<int, TEAM>{}, integral_constant<int, NV>{})
-    if (vec) {
-        if (dim <= 8 * V) SHAPE(V, 8, 1);
-        if (dim <= 16 * V) SHAPE(V, 16, 1);
-        if (dim <= 32 * V) SHAPE(V, 32, 1);
-        if (dim <= 64 * V) SHAPE(V, 32, 2);
-        if (dim <= 128 * V) SHAPE(V, 32, 4);
-        if (dim <= 512 * V) SHAPE(V, 256, 2);
-        if (dim <= 1024 * V) SHAPE(V, 256, 4);
-        if (dim <= 2048 * V) SHAPE(V, 256, 8);
-        SHAPE(V, 256, 64 / V);
-    }
-    if (dim <= 64) SHAPE(1, 16, 4);
-    if (dim <= 256) SHAPE(1, 32, 8);
-    if (dim <= 1024) SHAPE(1, 32, 32);
-    if (dim <= 4096) SHAPE(1, 256, 16);
-    SHAPE(1, 256, 64);
+#define SHAPE(TEAM, GROUPS)                                                                        \
+    return fast ? f(std::true_type{}, integral_constant<int, TEAM>{}, integral_constant<int, GROUPS>{}) \
+                : f(std::false_type{}, integral_constant<int, TEAM>{}, integral_constant<int, GROUPS>{})
+    if (dim <= 64) SHAPE(4, NV);
+    if (dim <= 128) SHAPE(8, NV);
+    if (dim <= 256) SHAPE(16, NV);
+    if (dim <= 512) SHAPE(32, NV);
+    if (dim <= 1024) SHAPE(64, NV);
+    if (dim <= 2048) SHAPE(128, NV);
+    if (dim <= 4096) SHAPE(256, NV);
+    if (dim <= 8192) SHAPE(256, 2 * NV);
+    SHAPE(256, 4 * NV);
 #undef SHAPE
 }
 
@@ -487,7 +623,7 @@ int with_type(int dtype, F&& f) {
     return f(float{});
 }
 
-// 16-byte groups: base and row pitch multiples of 16 bytes
+// base and row pitch multiples of 16 bytes
 bool vec_ok(const void* p, int64_t stride, int64_t es) {
     return !p || (((uintptr_t)p & 15) == 0 && (stride * es) % 16 == 0);
 }
@@ -517,8 +653,8 @@ bool bad_alias(const void* out, int64_t so, const void* in, int64_t si, int64_t 
 }
 
 // CTAs of the backward kernel: one partial sum each
-int back_ctas(const prism_ctx* ctx, int64_t rows, int teams) {
-    return (int)std::min<int64_t>((rows + teams - 1) / teams, (int64_t)ctx->sm_count * kBackCtasPerSm);
+int back_ctas(const prism_ctx* ctx, int64_t rows, int teams, int per_sm) {
+    return (int)std::min<int64_t>((rows + teams - 1) / teams, (int64_t)ctx->sm_count * per_sm);
 }
 
 }  // namespace
@@ -540,16 +676,17 @@ extern "C" int prism_layer_norm(prism_ctx* ctx, const prism_norm_params* p, cons
     if (bad_alias(y, p->y_stride, x, p->x_stride, p->rows, p->dim, es))
         return fail(PRISM_E_ARG, "prism_layer_norm: y overlaps x");
     DeviceGuard g(ctx->device);
-    NormArgs a{x, weight, bias, y, mean, rstd, p->rows, p->x_stride, p->y_stride, p->dim,
+    const int64_t xs = p->rows > 1 ? p->x_stride : p->dim, ys = p->rows > 1 ? p->y_stride : p->dim;
+    NormArgs a{x, weight, bias, y, mean, rstd, p->rows, xs, ys, p->dim,
                p->param_dtype == PRISM_DTYPE_F32, p->eps};
-    const bool vec = vec_ok(x, p->x_stride, es) && vec_ok(y, p->y_stride, es);
     return with_type(p->dtype, [&](auto tag) {
         using T = decltype(tag);
-        return with_shape<T>(vec, p->dim, [&](auto v, auto team, auto nv) {
+        const bool fast = p->dim % Pack<T>::N == 0 && vec_ok(x, xs, es) && vec_ok(y, ys, es);
+        return with_shape<T>(fast, p->dim, [&](auto quick, auto team, auto nv) {
             constexpr int kTeams = kThreads / decltype(team)::value;
             const int64_t want = (p->rows + kTeams - 1) / kTeams;
-            const int grid = (int)std::min<int64_t>(want, (int64_t)ctx->sm_count * 8);
-            norm_kernel<T, decltype(v)::value, decltype(team)::value, decltype(nv)::value>
+            const int grid = (int)std::min<int64_t>(want, (int64_t)ctx->sm_count * 3);
+            norm_kernel<decltype(quick)::value, T, decltype(team)::value, decltype(nv)::value>
                 <<<grid, kThreads, 0, as_stream(stream)>>>(a);
             return cuda_rc(cudaGetLastError(), "prism_layer_norm");
         });
@@ -597,24 +734,28 @@ extern "C" int prism_layer_norm_backward(prism_ctx* ctx, const prism_norm_params
     if (sums && (!workspace || workspace_bytes < need))
         return fail(PRISM_E_ARG, "%s: workspace of %zu bytes, %zu needed", who, workspace ? workspace_bytes : (size_t)0, need);
     if (sums && ((uintptr_t)workspace & 15)) return fail(PRISM_E_ALIGN, "%s: workspace is not 16-byte aligned", who);
+    const auto of = [&](int64_t stride) { return p->rows > 1 ? stride : (int64_t)p->dim; };
     NormBackArgs a{x,  weight, dy, add, mean, rstd, dx, sums ? static_cast<float*>(workspace) : nullptr,
-                   p->rows, p->x_stride, p->dy_stride, p->add_stride, p->dx_stride, p->dim,
+                   p->rows, of(p->x_stride), of(p->dy_stride), of(p->add_stride), of(p->dx_stride), p->dim,
                    p->param_dtype == PRISM_DTYPE_F32};
-    const bool vec = vec_ok(x, p->x_stride, es) && vec_ok(dy, p->dy_stride, es) && vec_ok(add, p->add_stride, es) &&
-                     vec_ok(dx, p->dx_stride, es);
     return with_type(p->dtype, [&](auto tag) {
         using T = decltype(tag);
         int grid = 0;
-        int rc = with_shape<T>(vec, p->dim, [&](auto v, auto team, auto nv) {
+        const bool fast = p->dim % Pack<T>::N == 0 && vec_ok(x, a.xs, es) && vec_ok(dy, a.dys, es) && vec_ok(add, a.adds, es) && vec_ok(dx, a.dxs, es);
+        int rc = with_shape<T>(fast, p->dim, [&](auto quick, auto team, auto nv) {
             constexpr int kTeam = decltype(team)::value;
-            grid = back_ctas(ctx, p->rows, kThreads / kTeam);
-            const size_t smem = sums && kTeam < kThreads ? (size_t)p->dim * 8 : 0;
-            norm_back_kernel<T, decltype(v)::value, kTeam, decltype(nv)::value>
-                <<<grid, kThreads, smem, as_stream(stream)>>>(a);
+            auto kernel = norm_back_kernel<decltype(quick)::value, T, kTeam, decltype(nv)::value>;
+            grid = back_ctas(ctx, p->rows, kThreads / kTeam, back_ctas_per_sm<decltype(quick)::value, T, decltype(nv)::value>());
+            const size_t smem = sums && kTeam < kThreads ? (size_t)(kTeam < 32 ? kWarps : kThreads / kTeam) * p->dim * 8 : 0;
+            if (smem > 40000) {
+                int e = cuda_rc(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+                if (e) return e;
+            }
+            kernel<<<grid, kThreads, smem, as_stream(stream)>>>(a);
             return cuda_rc(cudaGetLastError(), who);
         });
         if (rc || !sums) return rc;
-        return cuda_rc(launch_pdl(norm_fold_kernel<T>, dim3((2 * p->dim + 31) / 32), dim3(kThreads), 0, as_stream(stream),
+        return cuda_rc(launch_pdl(norm_fold_kernel<T>, dim3((2 * p->dim + 31) / 32), dim3(1024), 0, as_stream(stream),
                                   (const float*)workspace, grid, p->dim, dweight, dbias,
                                   (int)(p->param_dtype == PRISM_DTYPE_F32)),
                        who);

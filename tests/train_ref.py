@@ -78,9 +78,9 @@ def norm_back(x, w, mean, rstd, dy, add):
     if add is not None:
         dx = dx + add.double()
         t_dx = t_dx + 2 * U32 * (add.double().abs() + dx.abs())
-    # rows one after the other in a thread (at least 296 threads a column once there are that many
-    # rows, 2 CTAs on each of 148 SMs), then teams, warps and partial sums
-    k = R / 296 + 1 + 64
+    # rows one after the other in a thread (at least 148 threads a column, one on each SM, once there are
+    # that many rows), then the teams of a warp, the warps (13 together) and the CTAs' partial sums (10 + 32)
+    k = R / 148 + 1 + 64
     dw, db = (dy * xh).sum(0), dy.sum(0)
     t_dw = k * U32 * (dy * xh).abs().sum(0) + (dy.abs() * t_xh).sum(0)
     t_db = k * U32 * dy.abs().sum(0)
