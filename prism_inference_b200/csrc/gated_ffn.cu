@@ -11,7 +11,7 @@
 // K-major or MN-major is a bit of the MMA, so nothing is transposed.
 //   UP    [g | u] of 128 hidden columns side by side (the leader loads Wg, its peer Wu) -> h
 //   DOWN  y = h Wd^T
-//   BACK  [g | u] again from x, dh = dy Wd beside them -> dg, du, h
+//   BACK  dh = dy Wd and [g | u] again from x -> dg, du, h, and the bias gradients' sums on the way
 //   XW    dx tiles and dW tiles (split over rows) in one launch: neither fills the GPU alone
 // Rows go through in chunks, so the scratch memory does not grow with the batch.
 #include <cudaTypedefs.h>
@@ -25,16 +25,22 @@ namespace {
 
 enum Kind : int { UP, DOWN, BACK, XW };
 
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kStageA = 16384, kStageB = 16384, kStage = kStageA + kStageB;
-constexpr int kStages = 5;
-constexpr int kStageOut = 6144;  // a warp's store staging: three 32 x 32 16-bit boxes or one of fp32
-constexpr int kBiasBytes = kEpiWarps * 1024;
-constexpr int kSmem = kStages * kStage + kEpiWarps * kStageOut + kBiasBytes + 512 + 1024;
+constexpr int kOut = 4096;  // a warp's store staging: two 32 x 32 16-bit boxes or one of fp32
+// Epilogue warps and operand stages.  BACK's epilogue works out some 20 instructions a value between
+// its TMEM loads: 16 warps hide what 8 could not (13,000 cycles a unit against the MMAs' 3072).
+template <int KIND>
+struct Cfg {
+    static constexpr int kEpiWarps = KIND == BACK ? 16 : 8;
+    static constexpr int kThreads = 32 * (2 + kEpiWarps);
+    static constexpr int kStages = KIND == BACK ? 4 : 5;
+    static constexpr int kBias = KIND == BACK ? 256 : 512;  // bytes a warp
+    static constexpr int kSmem = kStages * kStage + kEpiWarps * (kOut + kBias) + 512 + 1024;
+};
+constexpr int kMaxStages = 5;
 
 struct Bars {
-    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     uint32_t tmem_base;
     int abort;
 };
@@ -49,7 +55,11 @@ struct Args {
     int bn;                     // N of an output tile over dim: 256 or 128
     int units, x_units;         // XW: the first x_units are dx tiles, the others dW tiles
     int w_tiles, k_per, k_all;  // XW: 256-row tiles of one weight's hidden axis; row blocks a split, in all
-    int act, bf16;
+    int act;
+    int first;                  // the first chunk: sums over rows start here
+    float *sums, *sums_dy;      // column sums of dg and du (BACK) and of dy (XW): [CTAs][4][2 hidden], [CTAs][4][dim]
+    const void* dy;             // XW: rows for the sums
+    int64_t dy_stride;
     const void *b_gate, *b_up, *b_down;
     const void* residual;
     int64_t residual_stride;
@@ -109,43 +119,72 @@ PRISM_DEV void gate_cols(const uint32_t (&g)[32], const uint32_t (&u)[32], const
         out[j] = pack2<T>(h0, h1);
     }
 }
-// dg over g's registers' first half, du, h: packed
+// 16 columns of one row: dg, du as fp32 pairs for the column sums, and all three packed
 template <typename T, int ACT>
-PRISM_DEV void grad_cols(const uint32_t (&g)[32], const uint32_t (&u)[32], const uint32_t (&dh)[32], const float* bg,
-                         const float* bu, uint32_t (&dg)[16], uint32_t (&du)[16], uint32_t (&h)[16]) {
+PRISM_DEV void grad_cols(const uint32_t (&g)[16], const uint32_t (&u)[16], const uint32_t (&dh)[16], const float* bg,
+                         const float* bu, uint64_t (&dg)[8], uint64_t (&du)[8], uint32_t* h) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const float2 b0 = reinterpret_cast<const float2*>(bg)[j], b1 = reinterpret_cast<const float2*>(bu)[j];
-        float pg[2], pu[2], ph[2];
+    for (int j = 0; j < 4; ++j) {
+        const ulonglong2 b0 = reinterpret_cast<const ulonglong2*>(bg)[j], b1 = reinterpret_cast<const ulonglong2*>(bu)[j];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float gv = __uint_as_float(g[2 * j + e]) + (e ? b0.y : b0.x);
-            const float uv = __uint_as_float(u[2 * j + e]) + (e ? b1.y : b1.x);
-            const float dv = __uint_as_float(dh[2 * j + e]);
-            float a, d;
-            gate_grad<ACT>(gv, a, d);
-            pg[e] = dv * uv * d;
-            pu[e] = dv * a;
-            ph[e] = a * uv;
+            const int i = 2 * j + e;
+            uint64_t hv;
+            gate_grad2<ACT>(f2_pack(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
+                            f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])),
+                            f2_pack(__uint_as_float(dh[2 * i]), __uint_as_float(dh[2 * i + 1])), e ? b0.y : b0.x, e ? b1.y : b1.x,
+                            dg[i], du[i], hv);
+            float h0, h1;
+            f2_unpack(hv, h0, h1);
+            h[i] = pack2<T>(h0, h1);
         }
-        dg[j] = pack2<T>(pg[0], pg[1]);
-        du[j] = pack2<T>(pu[0], pu[1]);
-        h[j] = pack2<T>(ph[0], ph[1]);
     }
+}
+template <typename T>
+PRISM_DEV uint4 pack8(const uint64_t* v) {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a, b;
+        f2_unpack(v[j], a, b);
+        o[j] = pack2<T>(a, b);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// Sums of 16 columns (as 8 pairs) over the warp's 32 rows: each step halves the columns that a lane still
+// holds (16 shuffles for 16 columns).  Lanes l and l + 1 end with column l / 2 (bits of l, high first).
+PRISM_DEV float column_sum(uint64_t (&v)[8], int lane) {
+#pragma unroll
+    for (int o = 4, bit = 16; o > 0; o >>= 1, bit >>= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const uint64_t send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = f2_add(keep, __shfl_xor_sync(0xffffffffu, send, bit));
+        }
+    }
+    float a, b;
+    f2_unpack(v[0], a, b);
+    const bool up = lane & 2;
+    a = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 2);
+    return a + __shfl_xor_sync(0xffffffffu, a, 1);
 }
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1, 1)
     gated_kernel(const Args a, const __grid_constant__ Maps maps) {
+    constexpr int kStages = Cfg<KIND>::kStages, kEpiWarps = Cfg<KIND>::kEpiWarps;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_align1k(smem_raw);
     unsigned char* s_out = smem + kStages * kStage;
-    float* s_bias = reinterpret_cast<float*>(s_out + kEpiWarps * kStageOut);
-    Bars* bars = reinterpret_cast<Bars*>(s_out + kEpiWarps * kStageOut + kBiasBytes);
+    unsigned char* s_bias = s_out + kEpiWarps * kOut;
+    Bars* bars = reinterpret_cast<Bars*>(s_bias + kEpiWarps * Cfg<KIND>::kBias);
     volatile int* abort = &bars->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    constexpr int kSlots = KIND == BACK ? 1 : 2;  // BACK's g | u | dh take 384 of the 512 columns
+    // Accumulators: two of 256 columns.  BACK has [g | u] in columns 0 .. 255 and dh in one of two slots
+    // of 128 behind them, so that a unit's dh is computed while the epilogue still reads the unit before.
+    constexpr int kSlots = KIND == BACK ? 1 : 2;
     constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
 
     if (threadIdx.x == 0) {
@@ -186,16 +225,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                     const uint32_t bar = peer_addr(smem_u32(&bars->full[stage]), 0);
                     uint32_t bytes;
                     const int row = t.mt * 256 + rank * 128;
-                    if (KIND == UP || (KIND == BACK && kb < kd)) {
+                    if (KIND == UP || (KIND == BACK && kb >= kd)) {
+                        const int k = (KIND == BACK ? kb - kd : kb) * 64;
                         bytes = kStageA + kStageB;
                         if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * bytes);
-                        tma_load_2d_pair(sa, &maps.a0, bar, kb * 64, row);
-                        tma_load_2d_pair(sb, rank ? &maps.b1 : &maps.b0, bar, kb * 64, t.nt * 128);
+                        tma_load_2d_pair(sa, &maps.a0, bar, k, row);
+                        tma_load_2d_pair(sb, rank ? &maps.b1 : &maps.b0, bar, k, t.nt * 128);
                     } else if (KIND == BACK) {
                         bytes = kStageA + kStageB / 2;
                         if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * bytes);
-                        tma_load_2d_pair(sa, &maps.a1, bar, (kb - kd) * 64, row);
-                        tma_load_2d_pair(sb, &maps.b2, bar, t.nt * 128 + rank * 64, (kb - kd) * 64);
+                        tma_load_2d_pair(sa, &maps.a1, bar, kb * 64, row);
+                        tma_load_2d_pair(sb, &maps.b2, bar, t.nt * 128 + rank * 64, kb * 64);
                     } else if (KIND == DOWN) {
                         bytes = kStageA + bh * 128;
                         if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * bytes);
@@ -235,12 +275,18 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                 const Unit t = unit_of<KIND>(a, u);
                 const int slot = it % kSlots;
                 const uint32_t acc = tmem + slot * 256;
-                if (!mbar_wait_cl(&bars->acc_empty[slot], ((it / kSlots) & 1) ^ 1, abort)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
+                if (KIND != BACK) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_cl(&bars->acc_empty[slot], ((it / kSlots) & 1) ^ 1, abort));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 const int kd = (a.dim + 63) / 64;
                 for (int kb = 0; kb < t.nkb; ++kb) {
+                    if (KIND == BACK && kb == kd) {  // dh is on its way; g and u need the last unit's read
+                        ok = __all_sync(0xffffffffu, mbar_wait_cl(&bars->acc_empty[0], (it & 1) ^ 1, abort));
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
                     if (!mbar_wait_w(&bars->full[stage], phase, abort)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + kStageA;
@@ -254,17 +300,18 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mma_pair_ss_w(acc, sdesc(sa + k * 32, SW128), sdesc_mn(sb + k * 2048, 8192), id, (kb | k) != 0);
-                    } else if (KIND == BACK && kb >= kd) {
+                    } else if (KIND == BACK && kb < kd) {
                         const uint32_t id = idesc_pair(256, 128, bf16, 0, 1);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc + 256, sdesc(sa + k * 32, SW128), sdesc_mn(sb + k * 2048, 8192), id,
-                                          (kb - kd) | k);
+                            mma_pair_ss_w(acc + 256 + (it & 1) * 128, sdesc(sa + k * 32, SW128), sdesc_mn(sb + k * 2048, 8192),
+                                          id, (kb | k) != 0);
                     } else {
                         const uint32_t id = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc, sdesc(sa + k * 32, SW128), sdesc(sb + k * 32, SW128), id, (kb | k) != 0);
+                            mma_pair_ss_w(acc, sdesc(sa + k * 32, SW128), sdesc(sb + k * 32, SW128), id,
+                                          (KIND == BACK ? (kb - kd) | k : kb | k) != 0);
                     }
                     mma_commit_pair_w(&bars->empty[stage]);
                     if (++stage == kStages) {
@@ -278,23 +325,50 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
     } else {
         // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .., half of the columns
+        // (a quarter in BACK)
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        unsigned char* buf = s_out + (warp - 2) * kStageOut;
+        unsigned char* buf = s_out + (warp - 2) * kOut;
         const uint32_t sbuf = smem_u32(buf);
-        float* bias = s_bias + (warp - 2) * 256;
+        float* bias = reinterpret_cast<float*>(s_bias + (warp - 2) * Cfg<KIND>::kBias);
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         const uint32_t acc_empty0 = peer_addr(smem_u32(&bars->acc_empty[0]), 0);
         const uint32_t acc_empty1 = peer_addr(smem_u32(&bars->acc_empty[1]), 0);
+        // Column sums of this warp's rows: BACK of dg and du, XW of dy.  Each warp has columns of its own.
+        float* sums = KIND == BACK ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden)
+                      : KIND == XW ? a.sums_dy + ((int64_t)blockIdx.x * 4 + quad) * a.dim : nullptr;
+        float next_g = 0.0f, next_u = 0.0f;  // BACK: the next unit's biases of column `lane`
+        if (KIND == BACK) {
+            if (a.first) {
+                for (int c = lane; c < a.hidden; c += 32)
+                    if (((c >> 5) & 3) == half) sums[c] = sums[a.hidden + c] = 0.0f;
+            }
+            const int c = pair % a.n_tiles * 128 + half * 32 + lane;
+            next_g = ld_bias<T>(a.b_gate, c, a.hidden);
+            next_u = ld_bias<T>(a.b_up, c, a.hidden);
+        }
+        if (KIND == XW && a.first) {
+            for (int c = lane; c < a.dim; c += 32)
+                if (((c >> 5) & 1) == half) sums[c] = 0.0f;
+        }
+        __syncwarp();
         int it = 0;
         for (int u = pair; u < a.units; u += pairs, ++it) {
             const Unit t = unit_of<KIND>(a, u);
             const int slot = it % kSlots;
             const int row = t.mt * 256 + rank * 128 + quad * 32;
-            constexpr bool kGate = KIND == UP || KIND == BACK;
-            const int cols = kGate ? 64 : a.bn / 2;  // this warp's
-            const int col0 = kGate ? t.nt * 128 + half * 64 : t.nt * a.bn + half * cols;
+            const int cols = KIND == BACK ? 32 : KIND == UP ? 64 : a.bn / 2;  // this warp's
+            const int col0 = (KIND == BACK || KIND == UP ? t.nt * 128 : t.nt * a.bn) + half * cols;
             // biases of this warp's columns
-            if (kGate) {
+            if (KIND == BACK) {
+                __syncwarp();
+                bias[lane] = next_g;
+                bias[32 + lane] = next_u;
+                const int c = (u + pairs) % a.n_tiles * 128 + half * 32 + lane;
+                if (u + pairs < a.units) {
+                    next_g = ld_bias<T>(a.b_gate, c, a.hidden);
+                    next_u = ld_bias<T>(a.b_up, c, a.hidden);
+                }
+            } else if (KIND == UP) {
                 for (int i = lane; i < 64; i += 32) {
                     bias[i] = ld_bias<T>(a.b_gate, col0 + i, a.hidden);
                     bias[64 + i] = ld_bias<T>(a.b_up, col0 + i, a.hidden);
@@ -302,51 +376,100 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             } else if (KIND == DOWN) {
                 for (int i = lane; i < cols; i += 32) bias[i] = ld_bias<T>(a.b_down, col0 + i, a.dim);
             }
+            if (KIND == XW && t.seg < 0 && t.nt == 0 && a.sums_dy) {  // while the unit's products run
+                const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
+                for (int c = half * 32; c < a.dim; c += 64) {
+                    const int cc = c + 2 * (lane & 15);
+                    uint32_t v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        v[i] = row + (lane >> 4) + 2 * i < a.rows && cc < a.dim
+                                   ? *reinterpret_cast<const uint32_t*>(dy + (int64_t)(2 * i) * a.dy_stride + cc) : 0u;
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float f0, f1;
+                        unpack2<T>(v[i], f0, f1);
+                        s0 += f0;
+                        s1 += f1;
+                    }
+                    s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
+                    s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
+                    if (cc < a.dim) atomicAdd(sums + cc + (lane >> 4), lane < 16 ? s0 : s1);
+                }
+            }
             __syncwarp();
             const bool got = mbar_wait_w(&bars->acc_full[slot], (it / kSlots) & 1, abort);
             if (!got) break;
             tc_fence_after();
             const uint32_t acc = tmem + lane_addr + slot * 256;
+            if (KIND == BACK) {
+                uint32_t h[16];
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int g = 0; g < 32; g += 16) {
+                    uint32_t rg[16], ru[16], rd[16];
+                    uint64_t dg[8], du[8];
+                    tmem_ld16(acc + half * 32 + g, rg);
+                    tmem_ld16(acc + 128 + half * 32 + g, ru);
+                    tmem_ld16(acc + 256 + (it & 1) * 128 + half * 32 + g, rd);
+                    tmem_ld_wait();
+                    if (g) {  // everything read: the next unit's products may come
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_peer(acc_empty0);
+                    }
+                    if (a.act == kActSilu) grad_cols<T, kActSilu>(rg, ru, rd, bias + g, bias + 32 + g, dg, du, h + g / 2);
+                    else if (a.act == kActGelu) grad_cols<T, kActGelu>(rg, ru, rd, bias + g, bias + 32 + g, dg, du, h + g / 2);
+                    else grad_cols<T, kActRelu>(rg, ru, rd, bias + g, bias + 32 + g, dg, du, h + g / 2);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        *reinterpret_cast<uint4*>(buf + sw64_off(lane, g / 8 + q)) = pack8<T>(dg + 4 * q);
+                        *reinterpret_cast<uint4*>(buf + 2048 + sw64_off(lane, g / 8 + q)) = pack8<T>(du + 4 * q);
+                    }
+                    // one warp adds to an address, in the order of its units: the same bits every time
+                    const float sg = column_sum(dg, lane), su = column_sum(du, lane);
+                    const int c = col0 + g + (lane >> 1);
+                    if (c < a.hidden) atomicAdd(sums + (lane & 1 ? a.hidden : 0) + c, lane & 1 ? su : sg);
+                }
+                const bool store = lane == 0 && col0 < a.hidden && row < a.rows;
+                fence_async_shared();
+                __syncwarp();
+                if (store) {
+                    tma_store_3d(&maps.out, sbuf, col0, row, 0);
+                    tma_store_3d(&maps.out, sbuf + 2048, col0, row, 1);
+                    tma_store_commit();
+                    tma_store_wait_read<0>();
+                }
+                __syncwarp();
+                stage_row64(buf, lane, h);
+                fence_async_shared();
+                __syncwarp();
+                if (store) {
+                    tma_store_3d(&maps.out, sbuf, col0, row, 2);
+                    tma_store_commit();
+                }
+                continue;
+            }
             for (int g = 0; g < cols; g += 32) {
                 const int c = col0 + g;
-                if (kGate) {
-                    uint32_t rg[32], ru[32];
+                if (KIND == UP) {
+                    uint32_t rg[32], ru[32], o[16];
                     tmem_ld32(acc + half * 64 + g, rg);
                     tmem_ld32(acc + 128 + half * 64 + g, ru);
-                    if (KIND == UP) {
-                        uint32_t o[16];
-                        tmem_ld_wait();
-                        if (a.act == kActSilu) gate_cols<T, kActSilu>(rg, ru, bias + g, bias + 64 + g, o);
-                        else if (a.act == kActGelu) gate_cols<T, kActGelu>(rg, ru, bias + g, bias + 64 + g, o);
-                        else gate_cols<T, kActRelu>(rg, ru, bias + g, bias + 64 + g, o);
-                        if (lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-                        stage_row64(buf, lane, o);
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0 && c < a.hidden && row < a.rows) {
-                            tma_store_2d(&maps.out, sbuf, c, row);
-                            tma_store_commit();
-                        }
-                    } else {
-                        uint32_t rd[32], dg[16], du[16], h[16];
-                        tmem_ld32(acc + 256 + half * 64 + g, rd);
-                        tmem_ld_wait();
-                        if (a.act == kActSilu) grad_cols<T, kActSilu>(rg, ru, rd, bias + g, bias + 64 + g, dg, du, h);
-                        else if (a.act == kActGelu) grad_cols<T, kActGelu>(rg, ru, rd, bias + g, bias + 64 + g, dg, du, h);
-                        else grad_cols<T, kActRelu>(rg, ru, rd, bias + g, bias + 64 + g, dg, du, h);
-                        if (lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-                        stage_row64(buf, lane, dg);
-                        stage_row64(buf + 2048, lane, du);
-                        stage_row64(buf + 4096, lane, h);
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0 && c < a.hidden && row < a.rows) {
-#pragma unroll
-                            for (int s = 0; s < 3; ++s) tma_store_3d(&maps.out, sbuf + 2048 * s, c, row, s);
-                            tma_store_commit();
-                        }
+                    tmem_ld_wait();
+                    if (a.act == kActSilu) gate_cols<T, kActSilu>(rg, ru, bias + g, bias + 64 + g, o);
+                    else if (a.act == kActGelu) gate_cols<T, kActGelu>(rg, ru, bias + g, bias + 64 + g, o);
+                    else gate_cols<T, kActRelu>(rg, ru, bias + g, bias + 64 + g, o);
+                    if (lane == 0) tma_store_wait_read<0>();
+                    __syncwarp();
+                    stage_row64(buf, lane, o);
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && c < a.hidden && row < a.rows) {
+                        tma_store_2d(&maps.out, sbuf, c, row);
+                        tma_store_commit();
                     }
                 } else {
                     uint32_t r[32];
@@ -362,7 +485,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                         fence_async_shared();
                         __syncwarp();
                         if (lane == 0 && c < a.dim && row < a.hidden) {
-                            tma_add_3d(&maps.dw, sbuf, c, row, t.split * 3 + t.seg);
+                            // one add to an address and launch: the same order, the same bits every time
+                            if (a.first) tma_store_3d(&maps.dw, sbuf, c, row, t.split * 3 + t.seg);
+                            else tma_add_3d(&maps.dw, sbuf, c, row, t.split * 3 + t.seg);
                             tma_store_commit();
                         }
                     } else {
@@ -413,61 +538,48 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// ---- column sums (bias gradients) ----------------------------------------------------------------
-// out[c] (+)= sum over rows of in[row][c], fp32: one CTA per 64 columns and row slice, 32 threads across
-// column pairs, 8 down the rows; partial sums [slice][cols].
+// ---- joining the partial sums ------------------------------------------------------------------
+// dW from the splits' sums [split][3][hidden][dim] by 32 x 32 tiles, the third weight transposed; behind
+// those CTAs, db from the warps' column sums [n_sums][2 hidden] and [n_dy][dim], 32 columns a CTA.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    col_sum_kernel(const T* in, int64_t stride, int rows, int cols, float* part, int first) {
-    __shared__ float2 red[8][32];
-    grid_dep_wait();
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int c = blockIdx.x * 64 + 2 * lane;
-    float s0 = 0.0f, s1 = 0.0f;
-    if (c < cols)
-        for (int r = blockIdx.y * 8 + k; r < rows; r += 8 * gridDim.y) {
-            float a, b;
-            unpack2<T>(*reinterpret_cast<const uint32_t*>(in + r * stride + c), a, b);
-            s0 += a;
-            s1 += b;
-        }
-    red[k][lane] = make_float2(s0, s1);
-    __syncthreads();
-    if (k == 0 && c < cols) {
-        s0 = s1 = 0.0f;
-        for (int i = 0; i < 8; ++i) {
-            s0 += red[i][lane].x;
-            s1 += red[i][lane].y;
-        }
-        float* p = part + (int64_t)blockIdx.y * cols + c;
-        p[0] = first ? s0 : p[0] + s0;
-        p[1] = first ? s1 : p[1] + s1;
-    }
-}
-template <typename T>
-__global__ void __launch_bounds__(256) col_fold_kernel(const float* part, int n_part, int cols, T* out) {
-    grid_dep_wait();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
-    float s = 0.0f;
-    for (int p = 0; p < n_part; ++p) s += part[(int64_t)p * cols + c];
-    out[c] = from_f32<T>(s);
-}
-
-// dW from the splits' sums [split][3][hidden][dim]: 32 x 32 tiles, the third weight transposed.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    dw_fold_kernel(const float* part, int splits, int hidden, int dim, T* dwg, T* dwu, T* dwd) {
+    fold_kernel(const float* dw, int splits, const float* sums, int n_sums, const float* sums_dy, int n_dy, int hidden, int dim,
+                T* dwg, T* dwu, T* dwd, T* dbg, T* dbu, T* dbd) {
     __shared__ float tile[32][33];
     grid_dep_wait();
-    const int seg = blockIdx.z, h0 = blockIdx.y * 32, d0 = blockIdx.x * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int dt = (dim + 31) / 32, ht = (hidden + 31) / 32;
+    int b = blockIdx.x;
+    if (b >= 3 * dt * ht) {
+        const int cols = 2 * hidden + dim, c = (b - 3 * dt * ht) * 32 + tx;
+        float s = 0.0f;
+        if (c < 2 * hidden)
+            for (int p = ty; p < n_sums; p += 8) s += sums[(int64_t)p * 2 * hidden + c];
+        else if (c < cols)
+            for (int p = ty; p < n_dy; p += 8) s += sums_dy[(int64_t)p * dim + c - 2 * hidden];
+        tile[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && c < cols) {
+            s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += tile[i][tx];
+            T* out = c < hidden ? dbg : c < 2 * hidden ? dbu : dbd;
+            if (out) out[c < hidden ? c : c < 2 * hidden ? c - hidden : c - 2 * hidden] = from_f32<T>(s);
+        }
+        return;
+    }
+    const int d0 = b % dt * 32;
+    b /= dt;
+    const int h0 = b % ht * 32, seg = b / ht;
     T* out = seg == 0 ? dwg : seg == 1 ? dwu : dwd;
     if (!out) return;
+#pragma unroll
     for (int i = ty; i < 32; i += 8) {
         const int h = h0 + i, d = d0 + tx;
         float s = 0.0f;
         if (h < hidden && d < dim) {
-            for (int k = 0; k < splits; ++k) s += part[(((int64_t)k * 3 + seg) * hidden + h) * dim + d];
+            const float* p = dw + ((int64_t)seg * hidden + h) * dim + d;
+            for (int k = 0; k < splits; ++k) s += p[(int64_t)k * 3 * hidden * dim];
             if (seg < 2) out[(int64_t)h * dim + d] = from_f32<T>(s);
         }
         tile[i][tx] = s;
@@ -525,10 +637,10 @@ constexpr CUtensorMapSwizzle kSw128 = CU_TENSOR_MAP_SWIZZLE_128B, kSw64 = CU_TEN
 template <typename T, int KIND>
 int launch(const prism_ctx* ctx, const Args& a, const Maps& m, cudaStream_t s, const char* who) {
     auto k = gated_kernel<T, KIND>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<KIND>::kSmem);
     if (e != cudaSuccess) return cuda_rc(e, who);
     const int pairs = std::min(a.units, ctx->sm_count / 2);
-    return cuda_rc(launch_pdl(k, dim3(2 * pairs), dim3(kThreads), kSmem, s, a, m), who);
+    return cuda_rc(launch_pdl(k, dim3(2 * pairs), dim3(Cfg<KIND>::kThreads), Cfg<KIND>::kSmem, s, a, m), who);
 }
 
 // Rows that go through at a time: a row tile for every CTA pair.
@@ -539,7 +651,7 @@ inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // scratch of the backward pass: p [3][rows][hidden] 16-bit, dw [splits][3][hidden][dim] fp32, column sums
 struct BackPlan {
     int64_t chunk;
-    int splits, slices;
+    int splits, pairs, pairs_xw;  // CTA pairs of the first chunk's launches: 8 rows of column sums each
     size_t p_bytes, dw_bytes, sum_bytes;
     size_t total() const { return p_bytes + dw_bytes + sum_bytes; }
 };
@@ -550,10 +662,12 @@ BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     const int64_t tiles = 3 * ((p->hidden + 255) / 256) * (int64_t)((p->dim + bn - 1) / bn);
     const int64_t kb = (b.chunk + 63) / 64;
     b.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kb, (ctx->sm_count / 2) / tiles));
-    b.slices = (int)std::max<int64_t>(1, std::min<int64_t>(64, b.chunk / 64));
+    b.pairs = (int)std::min<int64_t>(ctx->sm_count / 2, (b.chunk + 255) / 256 * ((p->hidden + 127) / 128));
+    const int64_t x_units = (b.chunk + 255) / 256 * ((p->dim + bn - 1) / bn), k_per = (kb + b.splits - 1) / b.splits;
+    b.pairs_xw = (int)std::min<int64_t>(ctx->sm_count / 2, x_units + tiles * ((kb + k_per - 1) / k_per));
     b.p_bytes = (size_t)up_to(3 * b.chunk * p->hidden * 2, 1024);
     b.dw_bytes = (size_t)up_to((int64_t)b.splits * 3 * p->hidden * p->dim * 4, 1024);
-    b.sum_bytes = (size_t)b.slices * (2 * (size_t)p->hidden + p->dim) * 4;
+    b.sum_bytes = (size_t)8 * (b.pairs * 2 * (size_t)p->hidden + b.pairs_xw * (size_t)p->dim) * 4;
     return b;
 }
 
@@ -641,10 +755,9 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
     const int64_t dxs = row_stride(p->dx_stride, p->rows, p->dim);
     T* pbuf = static_cast<T*>(ws);
     float* dw = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes);
-    float* sum_h = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes + b.dw_bytes);
-    float* sum_d = sum_h + (size_t)b.slices * 2 * p->hidden;
-    int rc;
-    if ((rc = cuda_rc(cudaMemsetAsync(dw, 0, b.dw_bytes, s), who))) return rc;
+    float* sums = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes + b.dw_bytes);
+    float* sums_dy = sums + (size_t)b.pairs * 8 * 2 * p->hidden;
+    int rc, splits = 1;
     for (int64_t r0 = 0; r0 < p->rows; r0 += b.chunk) {
         const int rows = (int)std::min(b.chunk, p->rows - r0);
         const T* xc = static_cast<const T*>(x) + r0 * xs;
@@ -657,6 +770,11 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
         a.b_gate = w->b_gate;
         a.b_up = w->b_up;
         a.err = ctx->err;
+        a.first = r0 == 0;
+        a.sums = sums;
+        a.sums_dy = sums_dy;
+        a.dy = dyc;
+        a.dy_stride = dys;
         a.bn = p->dim <= 128 ? 128 : 256;
         a.m_tiles = (rows + 255) / 256;
         a.n_tiles = (p->hidden + 127) / 128;
@@ -670,24 +788,14 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             (rc = make_map(&m.out, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 32, 32, kSw64)) ||
             (rc = launch<T, BACK>(ctx, a, m, s, who)))
             return rc;
-        // column sums of dg and du (one after the other in pbuf) and of dy
-        const dim3 gh((p->hidden + 63) / 64, b.slices), gd((p->dim + 63) / 64, b.slices);
-        for (int k = 0; k < 2; ++k)
-            if (k ? d->db_up : d->db_gate)
-                if ((rc = cuda_rc(launch_pdl(col_sum_kernel<T>, gh, dim3(256), 0, s, (const T*)(pbuf + (int64_t)k * rows * p->hidden),
-                                             (int64_t)p->hidden, rows, p->hidden, sum_h + (size_t)k * b.slices * p->hidden,
-                                             (int)(r0 == 0)), who)))
-                    return rc;
-        if (d->db_down && (rc = cuda_rc(launch_pdl(col_sum_kernel<T>, gd, dim3(256), 0, s, dyc, dys, rows, p->dim, sum_d,
-                                                   (int)(r0 == 0)), who)))
-            return rc;
         a.n_tiles = (p->dim + a.bn - 1) / a.bn;
         a.x_units = a.m_tiles * a.n_tiles;
         a.w_tiles = (p->hidden + 255) / 256;
         a.k_all = (rows + 63) / 64;
-        a.k_per = (a.k_all + b.splits - 1) / b.splits;
-        const int splits = (a.k_all + a.k_per - 1) / a.k_per;
-        a.units = a.x_units + 3 * a.w_tiles * a.n_tiles * splits;
+        a.k_per = (int)((up_to(b.chunk, 64) / 64 + b.splits - 1) / b.splits);
+        const int here = (a.k_all + a.k_per - 1) / a.k_per;
+        if (r0 == 0) splits = here;  // the first chunk is the largest: it writes every split's sums
+        a.units = a.x_units + 3 * a.w_tiles * a.n_tiles * here;
         if ((rc = make_map(&m.p_k, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 128, kSw128)) ||
             (rc = make_map(&m.p_mn, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 64, kSw128)) ||
             (rc = make_map(&m.b0, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
@@ -699,17 +807,11 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             (rc = launch<T, XW>(ctx, a, m, s, who)))
             return rc;
     }
-    if ((rc = cuda_rc(launch_pdl(dw_fold_kernel<T>, dim3((p->dim + 31) / 32, (p->hidden + 31) / 32, 3), dim3(256), 0, s,
-                                 (const float*)dw, b.splits, p->hidden, p->dim, static_cast<T*>(d->dw_gate),
-                                 static_cast<T*>(d->dw_up), static_cast<T*>(d->dw_down)), who)))
-        return rc;
-    const struct { void* out; const float* part; int cols; } sums[3] = {
-        {d->db_gate, sum_h, p->hidden}, {d->db_up, sum_h + (size_t)b.slices * p->hidden, p->hidden}, {d->db_down, sum_d, p->dim}};
-    for (const auto& f : sums)
-        if (f.out && (rc = cuda_rc(launch_pdl(col_fold_kernel<T>, dim3((f.cols + 255) / 256), dim3(256), 0, s, f.part, b.slices,
-                                              f.cols, static_cast<T*>(f.out)), who)))
-            return rc;
-    return PRISM_OK;
+    const int blocks = 3 * ((p->dim + 31) / 32) * ((p->hidden + 31) / 32) + (2 * p->hidden + p->dim + 31) / 32;
+    return cuda_rc(launch_pdl(fold_kernel<T>, dim3(blocks), dim3(256), 0, s, (const float*)dw, splits, (const float*)sums,
+                              b.pairs * 8, (const float*)sums_dy, b.pairs_xw * 8, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
+                              static_cast<T*>(d->dw_down), static_cast<T*>(d->db_gate), static_cast<T*>(d->db_up),
+                              static_cast<T*>(d->db_down)), who);
 }
 
 }  // namespace

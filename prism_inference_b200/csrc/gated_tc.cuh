@@ -99,24 +99,35 @@ PRISM_DEV float gate(float g) {
     const float z = g * fmaf(kGelu2c * kGeluA * kLog2e, g * g, kGelu2c * kLog2e);
     return g * sigmoid_exp2(z);
 }
-// act(g) and act'(g)
+PRISM_DEV uint64_t f2_same(float v) { return f2_pack(v, v); }
+// The gradient of two columns: from g, u (before their biases) and dh to dg, du and h, all in fp32
+// pairs (f32x2: the epilogue that runs this is bound by its instructions).
 template <int ACT>
-PRISM_DEV void gate_grad(float g, float& a, float& d) {
+PRISM_DEV void gate_grad2(uint64_t g, uint64_t u, uint64_t dh, uint64_t bg, uint64_t bu, uint64_t& dg, uint64_t& du, uint64_t& h) {
+    g = f2_add(g, bg);
+    u = f2_add(u, bu);
+    uint64_t a, d;  // act(g), act'(g)
     if (ACT == kActRelu) {
-        a = g <= 0.0f ? 0.0f : g;
-        d = g > 0.0f ? 1.0f : 0.0f;
-        return;
+        float g0, g1;
+        f2_unpack(g, g0, g1);
+        a = f2_pack(g0 <= 0.0f ? 0.0f : g0, g1 <= 0.0f ? 0.0f : g1);  // NaN stays
+        d = f2_pack(g0 > 0.0f ? 1.0f : 0.0f, g1 > 0.0f ? 1.0f : 0.0f);
+    } else {
+        const uint64_t g2 = f2_mul(g, g);
+        const uint64_t z = ACT == kActSilu ? f2_mul(g, f2_same(-kLog2e))
+                                           : f2_mul(g, f2_fma(f2_same(-kGelu2c * kGeluA * kLog2e), g2, f2_same(-kGelu2c * kLog2e)));
+        float z0, z1, e0, e1, s0, s1;
+        f2_unpack(z, z0, z1);
+        f2_unpack(f2_add(f2_pack(ex2_approx(z0), ex2_approx(z1)), f2_same(1.0f)), e0, e1);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(e0));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(e1));
+        const uint64_t s = f2_pack(s0, s1), r = f2_fma(s, f2_same(-1.0f), f2_same(1.0f));  // 1 - s
+        a = f2_mul(g, s);
+        d = ACT == kActSilu ? f2_fma(a, r, s) : f2_fma(f2_mul(a, r), f2_fma(f2_same(3.0f * kGelu2c * kGeluA), g2, f2_same(kGelu2c)), s);
     }
-    if (ACT == kActSilu) {
-        const float s = sigmoid_exp2(kLog2e * g);
-        a = g * s;
-        d = fmaf(a, 1.0f - s, s);
-        return;
-    }
-    const float g2 = g * g;
-    const float s = sigmoid_exp2(g * fmaf(kGelu2c * kGeluA * kLog2e, g2, kGelu2c * kLog2e));
-    a = g * s;
-    d = fmaf(a * (1.0f - s), fmaf(3.0f * kGelu2c * kGeluA, g2, kGelu2c), s);
+    dg = f2_mul(f2_mul(dh, u), d);
+    du = f2_mul(dh, a);
+    h = f2_mul(a, u);
 }
 
 }  // namespace prism
