@@ -18,7 +18,7 @@
 
 #include <algorithm>
 
-#include "gated_tc.cuh"
+#include "gated_fused.cuh"
 
 namespace prism {
 namespace {
@@ -119,57 +119,6 @@ PRISM_DEV void gate_cols(const uint32_t (&g)[32], const uint32_t (&u)[32], const
         out[j] = pack2<T>(h0, h1);
     }
 }
-// 16 columns of one row: dg, du as fp32 pairs for the column sums, and all three packed
-template <typename T, int ACT>
-PRISM_DEV void grad_cols(const uint32_t (&g)[16], const uint32_t (&u)[16], const uint32_t (&dh)[16], const float* bg,
-                         const float* bu, uint64_t (&dg)[8], uint64_t (&du)[8], uint32_t* h) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const ulonglong2 b0 = reinterpret_cast<const ulonglong2*>(bg)[j], b1 = reinterpret_cast<const ulonglong2*>(bu)[j];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = 2 * j + e;
-            uint64_t hv;
-            gate_grad2<ACT>(f2_pack(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
-                            f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])),
-                            f2_pack(__uint_as_float(dh[2 * i]), __uint_as_float(dh[2 * i + 1])), e ? b0.y : b0.x, e ? b1.y : b1.x,
-                            dg[i], du[i], hv);
-            float h0, h1;
-            f2_unpack(hv, h0, h1);
-            h[i] = pack2<T>(h0, h1);
-        }
-    }
-}
-template <typename T>
-PRISM_DEV uint4 pack8(const uint64_t* v) {
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float a, b;
-        f2_unpack(v[j], a, b);
-        o[j] = pack2<T>(a, b);
-    }
-    return make_uint4(o[0], o[1], o[2], o[3]);
-}
-// Sums of 16 columns (as 8 pairs) over the warp's 32 rows: each step halves the columns that a lane still
-// holds (16 shuffles for 16 columns).  Lanes l and l + 1 end with column l / 2 (bits of l, high first).
-PRISM_DEV float column_sum(uint64_t (&v)[8], int lane) {
-#pragma unroll
-    for (int o = 4, bit = 16; o > 0; o >>= 1, bit >>= 1) {
-        const bool up = lane & bit;
-#pragma unroll
-        for (int i = 0; i < o; ++i) {
-            const uint64_t send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
-            v[i] = f2_add(keep, __shfl_xor_sync(0xffffffffu, send, bit));
-        }
-    }
-    float a, b;
-    f2_unpack(v[0], a, b);
-    const bool up = lane & 2;
-    a = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 2);
-    return a + __shfl_xor_sync(0xffffffffu, a, 1);
-}
-
 template <typename T, int KIND>
 __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1, 1)
     gated_kernel(const Args a, const __grid_constant__ Maps maps) {
@@ -346,7 +295,7 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             next_g = ld_bias<T>(a.b_gate, c, a.hidden);
             next_u = ld_bias<T>(a.b_up, c, a.hidden);
         }
-        if (KIND == XW && a.first) {
+        if (KIND == XW && a.first && a.sums_dy) {
             for (int c = lane; c < a.dim; c += 32)
                 if (((c >> 5) & 1) == half) sums[c] = 0.0f;
         }
@@ -650,6 +599,7 @@ inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // scratch of the backward pass: p [3][rows][hidden] 16-bit, dw [splits][3][hidden][dim] fp32, column sums
 struct BackPlan {
+    bool fused;
     int64_t chunk;
     int splits, pairs, pairs_xw;  // CTA pairs of the first chunk's launches: 8 rows of column sums each
     size_t p_bytes, dw_bytes, sum_bytes;
@@ -662,9 +612,10 @@ BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     const int64_t tiles = 3 * ((p->hidden + 255) / 256) * (int64_t)((p->dim + bn - 1) / bn);
     const int64_t kb = (b.chunk + 63) / 64;
     b.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kb, (ctx->sm_count / 2) / tiles));
-    b.pairs = (int)std::min<int64_t>(ctx->sm_count / 2, (b.chunk + 255) / 256 * ((p->hidden + 127) / 128));
+    b.fused = p->dim <= kFusedMaxDim;
+    b.pairs = (int)std::min<int64_t>(ctx->sm_count / 2, (b.chunk + 255) / 256 * (b.fused ? 1 : (p->hidden + 127) / 128));
     const int64_t x_units = (b.chunk + 255) / 256 * ((p->dim + bn - 1) / bn), k_per = (kb + b.splits - 1) / b.splits;
-    b.pairs_xw = (int)std::min<int64_t>(ctx->sm_count / 2, x_units + tiles * ((kb + k_per - 1) / k_per));
+    b.pairs_xw = b.fused ? b.pairs : (int)std::min<int64_t>(ctx->sm_count / 2, x_units + tiles * ((kb + k_per - 1) / k_per));
     b.p_bytes = (size_t)up_to(3 * b.chunk * p->hidden * 2, 1024);
     b.dw_bytes = (size_t)up_to((int64_t)b.splits * 3 * p->hidden * p->dim * 4, 1024);
     b.sum_bytes = (size_t)8 * (b.pairs * 2 * (size_t)p->hidden + b.pairs_xw * (size_t)p->dim) * 4;
@@ -701,14 +652,51 @@ int check_weight(const char* who, const char* name, const void* t, bool needed, 
 }
 int64_t row_stride(int64_t stride, int64_t rows, int dim) { return rows > 1 ? stride : dim; }
 
+// rows of one fused forward launch: 32-bit row coordinates with room to spare
+constexpr int64_t kFusedRows = 1ll << 30;
+void fused_args(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, int rows, FusedArgs& a) {
+    a.rows = rows;
+    a.dim = p->dim;
+    a.hidden = p->hidden;
+    a.tiles = (rows + 255) / 256;
+    a.bn = p->dim <= 128 ? 128 : 256;
+    a.act = p->activation;
+    a.b_gate = w->b_gate;
+    a.b_up = w->b_up;
+    a.err = ctx->err;
+}
+int fused_maps(const prism_gated_params* p, const prism_gated_weights* w, const void* x, int64_t xs, int rows, int step, FusedMaps& m) {
+    int rc;
+    if ((rc = make_map(&m.x, x, p->dtype, p->dim, rows, 0, xs, 64, 128, kSw128)) ||
+        (rc = make_map(&m.wg, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, step, kSw128)))
+        return rc;
+    return make_map(&m.wu, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, step, kSw128);
+}
+
 template <typename T>
 int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
             const void* residual, void* y, void* ws, cudaStream_t s) {
     const char* who = "prism_gated_ffn";
-    const int64_t chunk = chunk_rows(ctx, p->rows);
     const int64_t xs = row_stride(p->x_stride, p->rows, p->dim), ys = row_stride(p->y_stride, p->rows, p->dim);
     const int64_t rs = row_stride(p->residual_stride, p->rows, p->dim);
     int rc;
+    // dim <= 256: one kernel; 522,240 x 256, hidden 1024: FWDNEW us against 1258 of the two that follow
+    for (int64_t r0 = 0; p->dim <= kFusedMaxDim && r0 < p->rows; r0 += kFusedRows) {
+        const int rows = (int)std::min(kFusedRows, p->rows - r0);
+        FusedArgs a = {};
+        FusedMaps m;
+        fused_args(ctx, p, w, rows, a);
+        a.b_down = w->b_down;
+        a.residual = residual ? static_cast<const T*>(residual) + r0 * rs : nullptr;
+        a.residual_stride = rs;
+        if ((rc = fused_maps(p, w, static_cast<const T*>(x) + r0 * xs, xs, rows, 128, m)) ||
+            (rc = make_map(&m.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 64, a.bn / 2, kSw128)) ||
+            (rc = make_map(&m.out, static_cast<T*>(y) + r0 * ys, p->dtype, p->dim, rows, 0, ys, 32, 32, kSw64)) ||
+            (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, false, a, m, ctx->sm_count, s), who)))
+            return rc;
+    }
+    if (p->dim <= kFusedMaxDim) return PRISM_OK;
+    const int64_t chunk = chunk_rows(ctx, p->rows);
     for (int64_t r0 = 0; r0 < p->rows; r0 += chunk) {
         const int rows = (int)std::min(chunk, p->rows - r0);
         const T* xc = static_cast<const T*>(x) + r0 * xs;
@@ -780,16 +768,38 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
         a.n_tiles = (p->hidden + 127) / 128;
         a.units = a.m_tiles * a.n_tiles;
         Maps m;
-        if ((rc = make_map(&m.a0, xc, p->dtype, p->dim, rows, 0, xs, 64, 128, kSw128)) ||
-            (rc = make_map(&m.a1, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
-            (rc = make_map(&m.b0, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 128, kSw128)) ||
-            (rc = make_map(&m.b1, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 128, kSw128)) ||
-            (rc = make_map(&m.b2, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 64, 64, kSw128)) ||
-            (rc = make_map(&m.out, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 32, 32, kSw64)) ||
-            (rc = launch<T, BACK>(ctx, a, m, s, who)))
-            return rc;
+        T* dxc = static_cast<T*>(dx) + r0 * dxs;
+        if (b.fused) {  // BFNEW us for 18,944 x 256, hidden 1024, against 62 of BACK and of XW's dx tiles
+            FusedArgs f = {};
+            FusedMaps fm;
+            fused_args(ctx, p, w, rows, f);
+            f.first = r0 == 0;
+            f.sums = sums;
+            f.sums_dy = sums_dy;
+            f.dy = dyc;
+            f.dy_stride = dys;
+            if ((rc = fused_maps(p, w, xc, xs, rows, 64, fm)) ||
+                (rc = make_map(&fm.dy, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
+                (rc = make_map(&fm.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 32, 128, kSw64)) ||
+                (rc = make_map(&fm.wg_mn, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
+                (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
+                (rc = make_map(&fm.p, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 32, kSw128)) ||
+                (rc = make_map(&fm.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
+                (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx->sm_count, s), who)))
+                return rc;
+            a.sums_dy = nullptr;
+        } else {
+            if ((rc = make_map(&m.a0, xc, p->dtype, p->dim, rows, 0, xs, 64, 128, kSw128)) ||
+                (rc = make_map(&m.a1, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
+                (rc = make_map(&m.b0, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 128, kSw128)) ||
+                (rc = make_map(&m.b1, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 128, kSw128)) ||
+                (rc = make_map(&m.b2, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 64, 64, kSw128)) ||
+                (rc = make_map(&m.out, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 32, 32, kSw64)) ||
+                (rc = launch<T, BACK>(ctx, a, m, s, who)))
+                return rc;
+        }
         a.n_tiles = (p->dim + a.bn - 1) / a.bn;
-        a.x_units = a.m_tiles * a.n_tiles;
+        a.x_units = b.fused ? 0 : a.m_tiles * a.n_tiles;
         a.w_tiles = (p->hidden + 255) / 256;
         a.k_all = (rows + 63) / 64;
         a.k_per = (int)((up_to(b.chunk, 64) / 64 + b.splits - 1) / b.splits);
@@ -802,7 +812,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             (rc = make_map(&m.b1, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
             (rc = make_map(&m.x_mn, xc, p->dtype, p->dim, rows, 0, xs, 64, 64, kSw128)) ||
             (rc = make_map(&m.dy_mn, dyc, p->dtype, p->dim, rows, 0, dys, 64, 64, kSw128)) ||
-            (rc = make_map(&m.out, static_cast<T*>(dx) + r0 * dxs, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
+            (rc = make_map(&m.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
             (rc = make_map(&m.dw, dw, PRISM_DTYPE_F32, p->dim, p->hidden, 3 * (int64_t)b.splits, p->dim, 32, 32, kSw128)) ||
             (rc = launch<T, XW>(ctx, a, m, s, who)))
             return rc;
@@ -823,7 +833,9 @@ extern "C" int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_param
     if (!ctx || !p || !bytes) return fail(PRISM_E_ARG, "prism_gated_ffn_workspace: NULL argument");
     int rc = check_gated("prism_gated_ffn_workspace", p);
     if (rc) return rc;
-    *bytes = p->rows == 0 ? 0 : backward ? back_plan(ctx, p).total() : (size_t)chunk_rows(ctx, p->rows) * p->hidden * 2;
+    *bytes = p->rows == 0                                    ? 0
+             : backward                                    ? back_plan(ctx, p).total()
+             : p->dim <= kFusedMaxDim ? 0 : (size_t)chunk_rows(ctx, p->rows) * p->hidden * 2;
     return PRISM_OK;
 }
 

@@ -1,0 +1,497 @@
+// gated_fused.cu - the gated feed-forward block for dim <= 256 as one kernel a direction.
+//
+// A CTA pair (tcgen05 cta_group::2) keeps 256 rows of x (backward: and dy) in shared memory and walks the
+// hidden layer in steps (128 columns forward, 64 backward, what TMEM and shared memory hold); the
+// hidden values never leave the SM forward.  Per step:
+//   forward   [g | u] = x [Wg | Wu]^T -> TMEM;  epilogue: h = act(g + bg) (u + bu) -> smem;  y += h Wd^T
+//   backward  [g | u] and dh = dy Wd -> TMEM;  epilogue: dg, du, h -> smem, from where TMA also stores
+//             them for the weight gradients' products, and column sums for the bias gradients;
+//             dx += dg Wg + du Wu
+// The MMA warp issues the products of step c + 1 before those that need the epilogue of step c, so the
+// tensor pipe works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3072
+// cycles of products), 80 KB backward (2850), some 30 bytes a clock; the streaming kernels of
+// gated_ffn.cu load every operand for every product and are held at the 37 to 40 that L2 gives an SM.
+#include <type_traits>
+
+#include "gated_fused.cuh"
+
+namespace prism {
+namespace {
+
+constexpr int kEpiWarps = 16;  // warp w: TMEM lanes 32 (w % 4) .., part (w - 2) / 4 of the columns
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kTile = 16384;  // 128 rows x 64 columns
+
+template <bool BWD>
+struct Cfg {
+    static constexpr int kStep = BWD ? 64 : 128;  // hidden columns a step
+    static constexpr int kCols = kStep / 4;       // of an epilogue warp
+    static constexpr int kRing = 3, kStage = BWD ? 16384 : 32768;
+    static constexpr int kXBytes = (BWD ? 8 : 4) * kTile;  // x, dy: four K-blocks each
+    static constexpr int kPBytes = (BWD ? 3 : 2) * kTile;  // dg, du, h, or h
+    static constexpr int kBias = 2 * kCols * 4;  // bytes a warp
+    // the dynamic shared memory of a kernel without static shared memory starts 1024-byte aligned
+    static constexpr int kSmem = kXBytes + kPBytes + kRing * kStage + kEpiWarps * kBias + 512;
+    static_assert(kSmem <= 232448, "227 KB");
+    static constexpr int kAcc = 256;  // first TMEM column of [g | u (| dh)], behind the output accumulator
+};
+struct Bars {
+    uint64_t full[3], empty[3], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
+    uint32_t tmem_base;
+    int abort;
+};
+
+template <typename T>
+PRISM_DEV float ld_bias(const void* b, int i, int n) {
+    return b && i < n ? to_f32(static_cast<const T*>(b)[i]) : 0.0f;
+}
+
+template <typename T, int ACT>
+PRISM_DEV void gate16(const uint32_t (&g)[16], const uint32_t (&u)[16], const float* bg, const float* bu, uint32_t (&h)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const ulonglong2 b0 = reinterpret_cast<const ulonglong2*>(bg)[j], b1 = reinterpret_cast<const ulonglong2*>(bu)[j];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = 2 * j + e;
+            float h0, h1;
+            f2_unpack(gate2<ACT>(f2_pack(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
+                                 f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), e ? b0.y : b0.x, e ? b1.y : b1.x),
+                      h0, h1);
+            h[i] = pack2<T>(h0, h1);
+        }
+    }
+}
+
+template <typename T, bool BWD>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    gated_fused_kernel(const FusedArgs a, const __grid_constant__ FusedMaps maps) {
+    using C = Cfg<BWD>;
+    extern __shared__ unsigned char smem[];
+    unsigned char* s_x = smem;
+    unsigned char* s_p = s_x + C::kXBytes;
+    unsigned char* s_ring = s_p + C::kPBytes;
+    unsigned char* s_bias = s_ring + C::kRing * C::kStage;
+    Bars* bars = reinterpret_cast<Bars*>(s_bias + kEpiWarps * C::kBias);
+    volatile int* abort = &bars->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    const int kd = (a.dim + 63) / 64, steps = (a.hidden + C::kStep - 1) / C::kStep;
+    const int bh = a.bn / 2;  // this CTA's share of N over dim
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kRing; ++s) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        mbar_init(&bars->x_full, 1);
+        mbar_init(&bars->y_full, 1);
+        mbar_init(&bars->x_empty, 1);
+        mbar_init(&bars->acc_full, 1);
+        mbar_init(&bars->acc_empty, 2 * kEpiWarps);  // those that epilogue warps arrive on: the leader's, both CTAs' warps
+        mbar_init(&bars->p_full, 2 * kEpiWarps);
+        mbar_init(&bars->p_empty, 1);
+        mbar_init(&bars->o_full, 1);
+        mbar_init(&bars->o_empty, 2 * kEpiWarps);
+        bars->abort = (smem_u32(smem) & 1023u) != 0;
+        fence_barrier_init();
+        fence_async_shared();
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc_pair(&bars->tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    grid_dep_wait();
+
+    if (warp == 0) {
+        // ---- producer (both CTAs)
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = !*abort;
+        // one ring stage of `bytes` a CTA: waits for room; true if this lane is to issue the loads
+        auto next = [&](uint32_t bytes, uint32_t& dst, uint32_t& bar) {
+            ok = ok && mbar_wait_w(&bars->empty[stage], phase ^ 1, abort);
+            dst = smem_u32(s_ring + stage * C::kStage);
+            bar = peer_addr(smem_u32(&bars->full[stage]), 0);
+            if (ok && lane == 0 && rank == 0) mbar_expect_tx(&bars->full[stage], 2 * bytes);
+            if (++stage == C::kRing) {
+                stage = 0;
+                phase ^= 1;
+            }
+            return ok && lane == 0;
+        };
+        uint32_t it = 0;
+        for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++it) {
+            const int row = tile * 256 + rank * 128;
+            ok = mbar_wait_w(&bars->x_empty, (it & 1) ^ 1, abort);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t bx = peer_addr(smem_u32(&bars->x_full), 0), by = peer_addr(smem_u32(&bars->y_full), 0);
+                if (rank == 0) {
+                    mbar_expect_tx(&bars->x_full, 2 * kd * kTile);
+                    if (BWD) mbar_expect_tx(&bars->y_full, 2 * kd * kTile);
+                }
+                for (int k = 0; k < kd; ++k) tma_load_2d_pair(smem_u32(s_x + k * kTile), &maps.x, bx, k * 64, row);
+                if (BWD)
+                    for (int k = 0; k < kd; ++k) tma_load_2d_pair(smem_u32(s_x + (4 + k) * kTile), &maps.dy, by, k * 64, row);
+            }
+            __syncwarp();
+            uint32_t dst, bar;
+            for (int c = 0; c <= steps && ok; ++c) {
+                if (c < steps) {
+                    // [g | u]: the leader brings Wg's rows, its peer Wu's; two K-blocks a stage
+                    for (int k = 0; k < kd; k += 2) {
+                        const int n = min(2, kd - k);
+                        if (next(n * C::kStep * 128, dst, bar))
+                            for (int i = 0; i < n; ++i)
+                                tma_load_2d_pair(dst + i * C::kStep * 128, rank ? &maps.wu : &maps.wg, bar, (k + i) * 64, c * C::kStep);
+                    }
+                    // dh: 128 rows of Wd (k) at a time, this CTA's 32 hidden columns (n)
+                    if (BWD && next((kd + 1) / 2 * 8192, dst, bar))
+                        for (int k = 0; k < kd; k += 2) tma_load_2d_pair(dst + k * 4096, &maps.wd, bar, c * 64 + rank * 32, k * 64);
+                }
+                if (c > 0 && !BWD) {  // y: this CTA's rows of Wd, both K-blocks of the step
+                    if (next(2 * bh * 128, dst, bar))
+                        for (int i = 0; i < 2; ++i) tma_load_2d_pair(dst + i * bh * 128, &maps.wd, bar, (c - 1) * 128 + i * 64, rank * bh);
+                }
+                if (c > 0 && BWD) {  // dx: the step's 64 hidden rows (k) of Wg, then Wu; this CTA's columns of dim (n)
+                    for (int s = 0; s < 2; ++s)
+                        if (next(bh * 128, dst, bar))
+                            for (int n = 0; n < bh; n += 64)
+                                tma_load_2d_pair(dst + n * 128, s ? &maps.wu_mn : &maps.wg_mn, bar, rank * bh + n, (c - 1) * 64);
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer: the leader's, for both CTAs
+        if (rank == 0) {
+            int stage = 0;
+            uint32_t phase = 0, it = 0, i = 0;  // i: steps so far
+            bool ok = !*abort;
+            auto take = [&](uint32_t& sb) {
+                ok = ok && mbar_wait_w(&bars->full[stage], phase, abort);
+                tc_fence_after();
+                sb = smem_u32(s_ring + stage * C::kStage);
+                return ok;
+            };
+            auto give = [&] {
+                mma_commit_pair_w(&bars->empty[stage]);
+                if (++stage == C::kRing) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            };
+            const uint32_t id_gu = idesc_pair(256, 2 * C::kStep, bf16, 0, 0), id_dh = idesc_pair(256, 64, bf16, 0, 1);
+            const uint32_t id_y = idesc_pair(256, a.bn, bf16, 0, 0), id_dx = idesc_pair(256, a.bn, bf16, 0, 1);
+            const uint32_t x_lo = desc_lo(smem_u32(s_x)), p_lo = desc_lo(smem_u32(s_p)), acc = tmem + C::kAcc;
+            constexpr uint32_t kBlk = kTile >> 4;
+            for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++it) {
+                ok = mbar_wait_w(&bars->x_full, it & 1, abort);
+                if (!ok) break;
+                for (int c = 0; c <= steps && ok; ++c) {
+                    uint32_t sb;
+                    if (c < steps) {
+                        // the epilogue has read the step before
+                        ok = mbar_wait_w(&bars->acc_empty, ((i + c) & 1) ^ 1, abort);
+                        if (!ok) break;
+                        for (int k = 0; k < kd; k += 2) {
+                            if (!take(sb)) break;
+                            const uint32_t b_lo = desc_lo(sb);
+                            mma_pair_x4<2, 2>(acc, x_lo + k * kBlk, kDescHi128, b_lo, kDescHi128, id_gu, k);
+                            if (k + 1 < kd)
+                                mma_pair_x4<2, 2>(acc, x_lo + (k + 1) * kBlk, kDescHi128, b_lo + C::kStep * 8, kDescHi128, id_gu, 1);
+                            give();
+                        }
+                        if (BWD && ok) {
+                            if (c == 0) {
+                                ok = mbar_wait_w(&bars->y_full, it & 1, abort);
+                                if (!ok) break;
+                            }
+                            if (!take(sb)) break;
+                            const uint32_t b_lo = desc_lo(sb);
+                            for (int k = 0; k < kd; ++k)
+                                mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo + k * 256, kDescHi64, id_dh, k);
+                            give();
+                        }
+                        if (!ok) break;
+                        mma_commit_pair_w(&bars->acc_full);
+                        if (c == steps - 1) mma_commit_pair_w(&bars->x_empty);
+                    }
+                    if (c > 0) {
+                        if (c == 1) {  // the last tile's output has been read
+                            ok = mbar_wait_w(&bars->o_empty, (it & 1) ^ 1, abort);
+                            if (!ok) break;
+                        }
+                        ok = mbar_wait_w(&bars->p_full, (i + c - 1) & 1, abort);
+                        if (!ok) break;
+                        fence_async_shared();
+                        if (!BWD) {
+                            if (!take(sb)) break;
+                            const uint32_t b_lo = desc_lo(sb);
+                            mma_pair_x4<2, 2>(tmem, p_lo, kDescHi128, b_lo, kDescHi128, id_y, c - 1);
+                            mma_pair_x4<2, 2>(tmem, p_lo + kBlk, kDescHi128, b_lo + bh * 8, kDescHi128, id_y, 1);
+                            give();
+                        } else {
+                            for (int s = 0; s < 2; ++s) {
+                                if (!take(sb)) break;
+                                mma_pair_x4<2, 128>(tmem, p_lo + s * kBlk, kDescHi128, desc_lo(sb, 8192), kDescHi128, id_dx, (c - 1) | s);
+                                give();
+                            }
+                        }
+                        if (!ok) break;
+                        mma_commit_pair_w(&bars->p_empty);
+                        if (c == steps) mma_commit_pair_w(&bars->o_full);
+                    }
+                }
+                i += steps;
+            }
+        }
+    } else {
+        // ---- epilogue
+        constexpr int kBiasVals = C::kBias / 128;
+        const int quad = warp & 3, part = (warp - 2) >> 2;
+        const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+        unsigned char* buf = s_p + (warp - 2) * 2048;  // store staging, once the tile's steps are done
+        float* bias = reinterpret_cast<float*>(s_bias + (warp - 2) * C::kBias);
+        const uint32_t acc_empty = peer_addr(smem_u32(&bars->acc_empty), 0), o_empty = peer_addr(smem_u32(&bars->o_empty), 0);
+        const uint32_t p_full = peer_addr(smem_u32(&bars->p_full), 0);
+        // this warp's rows of column sums; it alone has its columns of them
+        float* sums = BWD ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden) : nullptr;
+        float* sums_dy = BWD ? a.sums_dy + ((int64_t)blockIdx.x * 4 + quad) * a.dim : nullptr;
+        if (BWD && a.first) {
+            for (int c = lane; c < a.hidden; c += 32)
+                if (((c >> 4) & 3) == part) sums[c] = sums[a.hidden + c] = 0.0f;
+            for (int c = lane; c < a.dim; c += 32)
+                if (((c >> 6) & 3) == part) sums_dy[c] = 0.0f;
+        }
+        __syncwarp();
+        // the biases of this warp's columns of a step, gate's then up's: a value or two a lane, loaded a step ahead
+        float next_bias[kBiasVals];
+        auto load_bias = [&](int step) {
+#pragma unroll
+            for (int j = 0; j < kBiasVals; ++j) {
+                const int k = lane + 32 * j;
+                next_bias[j] = ld_bias<T>(k < C::kCols ? a.b_gate : a.b_up, step * C::kStep + part * C::kCols + k % C::kCols, a.hidden);
+            }
+        };
+        load_bias(0);
+        // A wait that gives up does not end the loops: the warps meet at barriers (which are not bounded),
+        // so all of them walk on to the end, where every further wait gives up at once.
+        uint32_t it = 0, i = 0;
+        for (int tile = pair; tile < a.tiles; tile += pairs, ++it) {
+            const int row = tile * 256 + rank * 128 + quad * 32;
+            if (BWD) {  // dy's column sums, while the first products run: 64 columns a warp
+                const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
+                for (int c = part * 64; c < min(a.dim, part * 64 + 64); c += 32) {
+                    const int cc = c + 2 * (lane & 15);
+                    uint32_t v[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        v[r] = row + (lane >> 4) + 2 * r < a.rows && cc < a.dim
+                                   ? *reinterpret_cast<const uint32_t*>(dy + (int64_t)(2 * r) * a.dy_stride + cc) : 0u;
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float f0, f1;
+                        unpack2<T>(v[r], f0, f1);
+                        s0 += f0;
+                        s1 += f1;
+                    }
+                    s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
+                    s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
+                    if (cc < a.dim) atomicAdd(sums_dy + cc + (lane >> 4), lane < 16 ? s0 : s1);
+                }
+            }
+            for (int c = 0; c < steps; ++c, ++i) {
+                const int col = c * C::kStep + part * C::kCols;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < kBiasVals; ++j) bias[lane + 32 * j] = next_bias[j];
+                load_bias(c + 1 < steps ? c + 1 : 0);
+                __syncwarp();
+                mbar_wait_w(&bars->acc_full, i & 1, abort);
+                tc_fence_after();
+                const uint32_t acc = tmem + lane_addr + C::kAcc + part * C::kCols;
+                const int prow = quad * 32 + lane;
+                uint32_t rg[16], ru[16];
+                if (!BWD) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int g = 0; g < 32; g += 16) {
+                        tmem_ld16(acc + g, rg);
+                        tmem_ld16(acc + 128 + g, ru);
+                        tmem_ld_wait();
+                        if (g) {  // all read
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_pair(acc_empty);
+                        }
+                        uint32_t(&o)[8] = reinterpret_cast<uint32_t(&)[8]>(h[g / 2]);
+                        if (a.act == kActSilu) gate16<T, kActSilu>(rg, ru, bias + g, bias + 32 + g, o);
+                        else if (a.act == kActGelu) gate16<T, kActGelu>(rg, ru, bias + g, bias + 32 + g, o);
+                        else gate16<T, kActRelu>(rg, ru, bias + g, bias + 32 + g, o);
+                    }
+                    mbar_wait_w(&bars->p_empty, (i & 1) ^ 1, abort);  // y of the step before has read p
+                    if (c == 0) {  // and the stores of the tile before
+                        if (lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+                        named_bar_sync(5, 32 * kEpiWarps);
+                    }
+                    unsigned char* p = s_p + (part >> 1) * kTile;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4*>(p + sw128_off(prow, (part & 1) * 4 + q)) =
+                            make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(p_full);
+                } else {
+                    uint32_t rd[16], h[8];
+                    uint64_t dg[8], du[8];
+                    unsigned char* p = s_p;
+                    tmem_ld16(acc, rg);
+                    tmem_ld16(acc + 64, ru);
+                    tmem_ld16(acc + 128, rd);
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(acc_empty);
+                    if (a.act == kActSilu) grad_cols<T, kActSilu>(rg, ru, rd, bias, bias + 16, dg, du, h);
+                    else if (a.act == kActGelu) grad_cols<T, kActGelu>(rg, ru, rd, bias, bias + 16, dg, du, h);
+                    else grad_cols<T, kActRelu>(rg, ru, rd, bias, bias + 16, dg, du, h);
+                    // room in p: dx of the step before has read it, and so have the stores (all four warps'
+                    // of these rows; at a tile's start, every warp's staging of the tile before)
+                    mbar_wait_w(&bars->p_empty, (i & 1) ^ 1, abort);
+                    if (c == 0) {
+                        if (lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+                        named_bar_sync(5, 32 * kEpiWarps);
+                    } else {
+                        if (part == 0 && lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+                        named_bar_sync(1 + quad, 128);
+                    }
+                    const uint32_t o0 = sw128_off(prow, part * 2), o1 = sw128_off(prow, part * 2 + 1);
+                    *reinterpret_cast<uint4*>(p + o0) = pack8<T>(dg);
+                    *reinterpret_cast<uint4*>(p + o1) = pack8<T>(dg + 4);
+                    *reinterpret_cast<uint4*>(p + kTile + o0) = pack8<T>(du);
+                    *reinterpret_cast<uint4*>(p + kTile + o1) = pack8<T>(du + 4);
+                    *reinterpret_cast<uint4*>(p + 2 * kTile + o0) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(p + 2 * kTile + o1) = make_uint4(h[4], h[5], h[6], h[7]);
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(p_full);
+                    named_bar_sync(1 + quad, 128);
+                    if (part == 0 && lane == 0 && row < a.rows) {
+                        const uint32_t src = smem_u32(s_p + quad * 4096);
+#pragma unroll
+                        for (int s = 0; s < 3; ++s) tma_store_3d(&maps.p, src + s * kTile, c * 64, row, s);
+                        tma_store_commit();
+                    }
+                    // one warp adds to an address, in the order of its steps: the same bits every time
+                    const float sg = column_sum(dg, lane), su = column_sum(du, lane);
+                    const int cs = col + (lane >> 1);
+                    if (cs < a.hidden) atomicAdd(sums + (lane & 1 ? a.hidden : 0) + cs, lane & 1 ? su : sg);
+                }
+            }
+            // ---- the tile's output: 64 columns a warp (32 where bn is 128)
+            const int cols = a.bn / 4, col0 = part * cols;
+            uint4 res[8];
+            float down[2] = {0.0f, 0.0f};
+            if (!BWD) {
+                down[0] = ld_bias<T>(a.b_down, col0 + lane, a.dim);
+                if (cols > 32) down[1] = ld_bias<T>(a.b_down, col0 + 32 + lane, a.dim);
+            }
+            if (!BWD && a.residual) {  // in flight while the last products run
+                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + lane) * a.residual_stride + col0;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)  // dim is a multiple of 8: a group is inside or outside
+                    res[q] = row + lane < a.rows && 8 * q < cols && col0 + 8 * q < a.dim ? *reinterpret_cast<const uint4*>(r + 8 * q)
+                                                                                          : make_uint4(0, 0, 0, 0);
+            }
+            mbar_wait_w(&bars->o_full, it & 1, abort);
+            if (BWD) {  // p becomes staging: its last products are done, and its last stores have been read
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+                named_bar_sync(5, 32 * kEpiWarps);
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int g = 0; g < 64; g += 32) {
+                if (g >= cols) break;
+                uint32_t r[32], o[16];
+                tmem_ld32(tmem + lane_addr + col0 + g, r);
+                tmem_ld_wait();
+                if (g + 32 >= cols) {  // all read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(o_empty);
+                }
+                const int c = col0 + g;
+                if (!BWD) {
+                    if (a.b_down) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, down[g / 32], j));
+                    }
+                    if (a.residual) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint4 v = res[g / 8 + q];
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                float f0, f1;
+                                unpack2<T>(w[j], f0, f1);
+                                const int k = 8 * q + 2 * j;
+                                r[k] = __float_as_uint(__uint_as_float(r[k]) + f0);
+                                r[k + 1] = __float_as_uint(__uint_as_float(r[k + 1]) + f1);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0 && c < a.dim && row < a.rows) {
+                    tma_store_2d(&maps.out, smem_u32(buf), c, row);
+                    tma_store_commit();
+                }
+            }
+        }
+        if (lane == 0) tma_store_wait0();
+    }
+    if (*abort && lane == 0) atomicOr(a.err, ERR_TIMEOUT);
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+template <typename T, bool BWD>
+cudaError_t launch(const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStream_t s) {
+    auto k = gated_fused_kernel<T, BWD>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BWD>::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k, dim3(2 * fused_pairs(a.tiles, sm_count)), dim3(kThreads), Cfg<BWD>::kSmem, s, a, m);
+}
+
+}  // namespace
+
+cudaError_t launch_gated_fused(bool bf16, bool backward, const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStream_t s) {
+    if (bf16) return backward ? launch<__nv_bfloat16, true>(a, m, sm_count, s) : launch<__nv_bfloat16, false>(a, m, sm_count, s);
+    return backward ? launch<__half, true>(a, m, sm_count, s) : launch<__half, false>(a, m, sm_count, s);
+}
+
+}  // namespace prism

@@ -56,6 +56,39 @@ PRISM_DEV void mma_pair_ss_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, ui
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Matrix descriptors as (low, high) words: the low word holds the address, so the operands of one MMA
+// after another differ by an addition there.
+PRISM_DEV uint32_t desc_lo(uint32_t saddr, uint32_t group_bytes = 16) { return (saddr >> 4) | (group_bytes >> 4) << 16; }
+constexpr uint32_t kDescHi128 = (1024u >> 4) | (1u << 14) | ((uint32_t)SW128 << 29);
+constexpr uint32_t kDescHi64 = (512u >> 4) | (1u << 14) | ((uint32_t)SW64 << 29);
+// Four MMAs (64 deep) whose descriptors advance by ASTEP, BSTEP 16-byte units, the first one adding to D
+// if `accumulate`.  One block, one elect: issued one by one, with their descriptors worked out each
+// time, 16 MMAs of N = 128 took 2000 cycles to issue for 1072 cycles of work.
+template <int ASTEP, int BSTEP>
+PRISM_DEV void mma_pair_x4(uint32_t d_tmem, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e, t;\n\t.reg .b32 r, a1, a2, a3, b1, b2, b3;\n\t.reg .b64 x0, x1, x2, x3, y0, y1, y2, y3;\n\t"
+        "add.u32 a1, %1, %7;\n\tadd.u32 a2, %1, %8;\n\tadd.u32 a3, %1, %9;\n\t"
+        "add.u32 b1, %3, %10;\n\tadd.u32 b2, %3, %11;\n\tadd.u32 b3, %3, %12;\n\t"
+        "mov.b64 x0, {%1, %2};\n\tmov.b64 x1, {a1, %2};\n\tmov.b64 x2, {a2, %2};\n\tmov.b64 x3, {a3, %2};\n\t"
+        "mov.b64 y0, {%3, %4};\n\tmov.b64 y1, {b1, %4};\n\tmov.b64 y2, {b2, %4};\n\tmov.b64 y3, {b3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.eq.u32 t, 0, 0;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x0, y0, %5, p;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x1, y1, %5, t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x2, y2, %5, t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x3, y3, %5, t;\n\t}" ::"r"(d_tmem),
+        "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "n"(ASTEP), "n"(2 * ASTEP), "n"(3 * ASTEP),
+        "n"(BSTEP), "n"(2 * BSTEP), "n"(3 * BSTEP)
+        : "memory");
+}
+// Arrives on an mbarrier of this CTA or its peer (a shared::cluster address).  What is handed over is
+// shared memory that the tensor core reads (made visible by fence.proxy.async before) or TMEM (by
+// tcgen05.fence), so the arrival itself carries no cluster-scope release, which costs a full memory
+// barrier: 40 -> 33 us for 8160 rows forward.
+PRISM_DEV void mbar_arrive_pair(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
 // arrives on the barrier at this offset in both CTAs once every MMA issued before has completed
 PRISM_DEV void mma_commit_pair_w(uint64_t* bar) {
     asm volatile(
@@ -100,6 +133,23 @@ PRISM_DEV float gate(float g) {
     return g * sigmoid_exp2(z);
 }
 PRISM_DEV uint64_t f2_same(float v) { return f2_pack(v, v); }
+// act(g + bg) (u + bu) of two columns
+template <int ACT>
+PRISM_DEV uint64_t gate2(uint64_t g, uint64_t u, uint64_t bg, uint64_t bu) {
+    g = f2_add(g, bg);
+    u = f2_add(u, bu);
+    float g0, g1;
+    f2_unpack(g, g0, g1);
+    if (ACT == kActRelu) return f2_mul(f2_pack(g0 <= 0.0f ? 0.0f : g0, g1 <= 0.0f ? 0.0f : g1), u);  // NaN stays
+    const uint64_t z = ACT == kActSilu ? f2_mul(g, f2_same(-kLog2e))
+                                       : f2_mul(g, f2_fma(f2_same(-kGelu2c * kGeluA * kLog2e), f2_mul(g, g), f2_same(-kGelu2c * kLog2e)));
+    float z0, z1, e0, e1, s0, s1;
+    f2_unpack(z, z0, z1);
+    f2_unpack(f2_add(f2_pack(ex2_approx(z0), ex2_approx(z1)), f2_same(1.0f)), e0, e1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(e0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(e1));
+    return f2_mul(f2_mul(g, f2_pack(s0, s1)), u);
+}
 // The gradient of two columns: from g, u (before their biases) and dh to dg, du and h, all in fp32
 // pairs (f32x2: the epilogue that runs this is bound by its instructions).
 template <int ACT>
@@ -128,6 +178,57 @@ PRISM_DEV void gate_grad2(uint64_t g, uint64_t u, uint64_t dh, uint64_t bg, uint
     dg = f2_mul(f2_mul(dh, u), d);
     du = f2_mul(dh, a);
     h = f2_mul(a, u);
+}
+
+// 16 columns of one row: dg, du as fp32 pairs for the column sums, and all three packed
+template <typename T, int ACT>
+PRISM_DEV void grad_cols(const uint32_t (&g)[16], const uint32_t (&u)[16], const uint32_t (&dh)[16], const float* bg,
+                         const float* bu, uint64_t (&dg)[8], uint64_t (&du)[8], uint32_t* h) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const ulonglong2 b0 = reinterpret_cast<const ulonglong2*>(bg)[j], b1 = reinterpret_cast<const ulonglong2*>(bu)[j];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = 2 * j + e;
+            uint64_t hv;
+            gate_grad2<ACT>(f2_pack(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
+                            f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])),
+                            f2_pack(__uint_as_float(dh[2 * i]), __uint_as_float(dh[2 * i + 1])), e ? b0.y : b0.x, e ? b1.y : b1.x,
+                            dg[i], du[i], hv);
+            float h0, h1;
+            f2_unpack(hv, h0, h1);
+            h[i] = pack2<T>(h0, h1);
+        }
+    }
+}
+template <typename T>
+PRISM_DEV uint4 pack8(const uint64_t* v) {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a, b;
+        f2_unpack(v[j], a, b);
+        o[j] = pack2<T>(a, b);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// Sums of 16 columns (as 8 pairs) over the warp's 32 rows: each step halves the columns that a lane still
+// holds (16 shuffles for 16 columns).  Lanes l and l + 1 end with column l / 2 (bits of l, high first).
+PRISM_DEV float column_sum(uint64_t (&v)[8], int lane) {
+#pragma unroll
+    for (int o = 4, bit = 16; o > 0; o >>= 1, bit >>= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const uint64_t send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = f2_add(keep, __shfl_xor_sync(0xffffffffu, send, bit));
+        }
+    }
+    float a, b;
+    f2_unpack(v[0], a, b);
+    const bool up = lane & 2;
+    a = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 2);
+    return a + __shfl_xor_sync(0xffffffffu, a, 1);
 }
 
 }  // namespace prism

@@ -238,8 +238,12 @@ def test_refusals(prism_ctx):
         forward(prism_ctx, wide[:, :D], w, b, wide[:, 32:32 + D])
     with pytest.raises(PrismError, match="ALIGN"):
         forward(prism_ctx, wide[:, 1:1 + D], w, b, y)
+    small = torch.empty(16, dtype=torch.uint8, device="cuda")
     with pytest.raises(PrismError, match="workspace"):
-        forward(prism_ctx, x, w, b, y, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+        backward(prism_ctx, x, w, b, y, torch.empty_like(x), {}, workspace=small)
+    with pytest.raises(PrismError, match="workspace"):  # the forward pass needs one above dim 256
+        x2, (w2, b2) = rand((4, 264), F16, 1), weights(264, H, F16)
+        forward(prism_ctx, x2, w2, b2, torch.empty_like(x2), workspace=small)
     with pytest.raises(PrismError, match="overlaps"):
         backward(prism_ctx, x, w, b, y, y, {})
     for bad in (lambda: forward(prism_ctx, x, w, b, y, activation="tanh"), lambda: forward(prism_ctx, x, w, b, y.bfloat16()),
