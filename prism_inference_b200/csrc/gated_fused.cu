@@ -19,11 +19,12 @@ namespace prism {
 namespace {
 
 constexpr int kEpiWarps = 16;  // warp w: TMEM lanes 32 (w % 4) .., part (w - 2) / 4 of the columns
-constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr int kTile = 16384;  // 128 rows x 64 columns
+constexpr int kTile = 16384;   // 128 rows x 64 columns
 
 template <bool BWD>
 struct Cfg {
+    // producer, MMA issuer, epilogue warps; backward, a last one that stores p
+    static constexpr int kThreads = 32 * (2 + kEpiWarps + BWD);
     static constexpr int kStep = BWD ? 64 : 128;  // hidden columns a step
     static constexpr int kCols = kStep / 4;       // of an epilogue warp
     static constexpr int kRing = 3, kStage = BWD ? 16384 : 32768;
@@ -37,6 +38,7 @@ struct Cfg {
 };
 struct Bars {
     uint64_t full[3], empty[3], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
+    uint64_t p_quad[4], p_read;  // backward: a quad's rows of p are written; p's stores have read it
     uint32_t tmem_base;
     int abort;
 };
@@ -47,9 +49,9 @@ PRISM_DEV float ld_bias(const void* b, int i, int n) {
 }
 
 template <typename T, int ACT>
-PRISM_DEV void gate16(const uint32_t (&g)[16], const uint32_t (&u)[16], const float* bg, const float* bu, uint32_t (&h)[8]) {
+PRISM_DEV void gate32(const uint32_t (&g)[32], const uint32_t (&u)[32], const float* bg, const float* bu, uint32_t (&h)[16]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
         const ulonglong2 b0 = reinterpret_cast<const ulonglong2*>(bg)[j], b1 = reinterpret_cast<const ulonglong2*>(bu)[j];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -64,7 +66,7 @@ PRISM_DEV void gate16(const uint32_t (&g)[16], const uint32_t (&u)[16], const fl
 }
 
 template <typename T, bool BWD>
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 1)
     gated_fused_kernel(const FusedArgs a, const __grid_constant__ FusedMaps maps) {
     using C = Cfg<BWD>;
     extern __shared__ unsigned char smem[];
@@ -94,6 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         mbar_init(&bars->p_empty, 1);
         mbar_init(&bars->o_full, 1);
         mbar_init(&bars->o_empty, 2 * kEpiWarps);
+        for (int q = 0; q < 4; ++q) mbar_init(&bars->p_quad[q], 4);
+        mbar_init(&bars->p_read, 1);
         bars->abort = (smem_u32(smem) & 1023u) != 0;
         fence_barrier_init();
         fence_async_shared();
@@ -173,11 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             int stage = 0;
             uint32_t phase = 0, it = 0, i = 0;  // i: steps so far
             bool ok = !*abort;
-            auto take = [&](uint32_t& sb) {
-                ok = ok && mbar_wait_w(&bars->full[stage], phase, abort);
+            auto take = [&] {
+                mbar_wait_step(&bars->full[stage], phase, abort);
                 tc_fence_after();
-                sb = smem_u32(s_ring + stage * C::kStage);
-                return ok;
+                return smem_u32(s_ring + stage * C::kStage);
             };
             auto give = [&] {
                 mma_commit_pair_w(&bars->empty[stage]);
@@ -191,59 +194,44 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             const uint32_t x_lo = desc_lo(smem_u32(s_x)), p_lo = desc_lo(smem_u32(s_p)), acc = tmem + C::kAcc;
             constexpr uint32_t kBlk = kTile >> 4;
             for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++it) {
-                ok = mbar_wait_w(&bars->x_full, it & 1, abort);
-                if (!ok) break;
-                for (int c = 0; c <= steps && ok; ++c) {
-                    uint32_t sb;
+                mbar_wait_step(&bars->x_full, it & 1, abort);
+                for (int c = 0; c <= steps; ++c) {
+                    ok = __all_sync(0xffffffffu, !*abort);
+                    if (!ok) break;
                     if (c < steps) {
                         // the epilogue has read the step before
-                        ok = mbar_wait_w(&bars->acc_empty, ((i + c) & 1) ^ 1, abort);
-                        if (!ok) break;
+                        mbar_wait_step(&bars->acc_empty, ((i + c) & 1) ^ 1, abort);
                         for (int k = 0; k < kd; k += 2) {
-                            if (!take(sb)) break;
-                            const uint32_t b_lo = desc_lo(sb);
+                            const uint32_t b_lo = desc_lo(take());
                             mma_pair_x4<2, 2>(acc, x_lo + k * kBlk, kDescHi128, b_lo, kDescHi128, id_gu, k);
                             if (k + 1 < kd)
                                 mma_pair_x4<2, 2>(acc, x_lo + (k + 1) * kBlk, kDescHi128, b_lo + C::kStep * 8, kDescHi128, id_gu, 1);
                             give();
                         }
-                        if (BWD && ok) {
-                            if (c == 0) {
-                                ok = mbar_wait_w(&bars->y_full, it & 1, abort);
-                                if (!ok) break;
-                            }
-                            if (!take(sb)) break;
-                            const uint32_t b_lo = desc_lo(sb);
+                        if (BWD) {
+                            if (c == 0) mbar_wait_step(&bars->y_full, it & 1, abort);
+                            const uint32_t b_lo = desc_lo(take());
                             for (int k = 0; k < kd; ++k)
                                 mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo + k * 256, kDescHi64, id_dh, k);
                             give();
                         }
-                        if (!ok) break;
                         mma_commit_pair_w(&bars->acc_full);
                         if (c == steps - 1) mma_commit_pair_w(&bars->x_empty);
                     }
                     if (c > 0) {
-                        if (c == 1) {  // the last tile's output has been read
-                            ok = mbar_wait_w(&bars->o_empty, (it & 1) ^ 1, abort);
-                            if (!ok) break;
-                        }
-                        ok = mbar_wait_w(&bars->p_full, (i + c - 1) & 1, abort);
-                        if (!ok) break;
-                        fence_async_shared();
+                        if (c == 1) mbar_wait_step(&bars->o_empty, (it & 1) ^ 1, abort);  // the last tile's output has been read
+                        mbar_wait_step(&bars->p_full, (i + c - 1) & 1, abort);
                         if (!BWD) {
-                            if (!take(sb)) break;
-                            const uint32_t b_lo = desc_lo(sb);
+                            const uint32_t b_lo = desc_lo(take());
                             mma_pair_x4<2, 2>(tmem, p_lo, kDescHi128, b_lo, kDescHi128, id_y, c - 1);
                             mma_pair_x4<2, 2>(tmem, p_lo + kBlk, kDescHi128, b_lo + bh * 8, kDescHi128, id_y, 1);
                             give();
                         } else {
                             for (int s = 0; s < 2; ++s) {
-                                if (!take(sb)) break;
-                                mma_pair_x4<2, 128>(tmem, p_lo + s * kBlk, kDescHi128, desc_lo(sb, 8192), kDescHi128, id_dx, (c - 1) | s);
+                                mma_pair_x4<2, 128>(tmem, p_lo + s * kBlk, kDescHi128, desc_lo(take(), 8192), kDescHi128, id_dx, (c - 1) | s);
                                 give();
                             }
                         }
-                        if (!ok) break;
                         mma_commit_pair_w(&bars->p_empty);
                         if (c == steps) mma_commit_pair_w(&bars->o_full);
                     }
@@ -251,6 +239,28 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                 i += steps;
             }
         }
+    } else if (BWD && warp == 2 + kEpiWarps) {
+        // ---- stores of p: 32 rows as soon as their four warps have written them
+        uint32_t i = 0;
+        for (int tile = pair; tile < a.tiles; tile += pairs)
+            for (int c = 0; c < steps; ++c, ++i) {
+                for (int q = 0; q < 4; ++q) {
+                    mbar_wait_step(&bars->p_quad[q], i & 1, abort);
+                    const int row = tile * 256 + rank * 128 + q * 32;
+                    if (lane == 0 && row < a.rows) {
+                        const uint32_t src = smem_u32(s_p + q * 4096);
+#pragma unroll
+                        for (int s = 0; s < 3; ++s) tma_store_3d(&maps.p, src + s * kTile, c * 64, row, s);
+                    }
+                }
+                if (lane == 0) {
+                    tma_store_commit();
+                    tma_store_wait_read<0>();
+                    mbar_arrive(&bars->p_read);
+                }
+                __syncwarp();
+            }
+        if (lane == 0) tma_store_wait0();
     } else {
         // ---- epilogue
         constexpr int kBiasVals = C::kBias / 128;
@@ -285,6 +295,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         uint32_t it = 0, i = 0;
         for (int tile = pair; tile < a.tiles; tile += pairs, ++it) {
             const int row = tile * 256 + rank * 128 + quad * 32;
+            if (!BWD && a.residual && row + lane < a.rows && part * a.bn / 4 < a.dim) {  // on its way to L2: this warp's columns, a line at most
+                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + lane) * a.residual_stride + part * a.bn / 4;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(r));
+            }
             if (BWD) {  // dy's column sums, while the first products run: 64 columns a warp
                 const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
                 for (int c = part * 64; c < min(a.dim, part * 64 + 64); c += 32) {
@@ -318,24 +332,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                 tc_fence_after();
                 const uint32_t acc = tmem + lane_addr + C::kAcc + part * C::kCols;
                 const int prow = quad * 32 + lane;
-                uint32_t rg[16], ru[16];
                 if (!BWD) {
-                    uint32_t h[16];
-#pragma unroll
-                    for (int g = 0; g < 32; g += 16) {
-                        tmem_ld16(acc + g, rg);
-                        tmem_ld16(acc + 128 + g, ru);
-                        tmem_ld_wait();
-                        if (g) {  // all read
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_pair(acc_empty);
-                        }
-                        uint32_t(&o)[8] = reinterpret_cast<uint32_t(&)[8]>(h[g / 2]);
-                        if (a.act == kActSilu) gate16<T, kActSilu>(rg, ru, bias + g, bias + 32 + g, o);
-                        else if (a.act == kActGelu) gate16<T, kActGelu>(rg, ru, bias + g, bias + 32 + g, o);
-                        else gate16<T, kActRelu>(rg, ru, bias + g, bias + 32 + g, o);
-                    }
+                    uint32_t rg[32], ru[32], h[16];
+                    tmem_ld32(acc, rg);
+                    tmem_ld32(acc + 128, ru);
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(acc_empty);  // the next step's products may come
+                    if (a.act == kActSilu) gate32<T, kActSilu>(rg, ru, bias, bias + 32, h);
+                    else if (a.act == kActGelu) gate32<T, kActGelu>(rg, ru, bias, bias + 32, h);
+                    else gate32<T, kActRelu>(rg, ru, bias, bias + 32, h);
                     mbar_wait_w(&bars->p_empty, (i & 1) ^ 1, abort);  // y of the step before has read p
                     if (c == 0) {  // and the stores of the tile before
                         if (lane == 0) tma_store_wait_read<0>();
@@ -351,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_pair(p_full);
                 } else {
-                    uint32_t rd[16], h[8];
+                    uint32_t rg[16], ru[16], rd[16], h[8];
                     uint64_t dg[8], du[8];
                     unsigned char* p = s_p;
                     tmem_ld16(acc, rg);
@@ -364,17 +371,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                     if (a.act == kActSilu) grad_cols<T, kActSilu>(rg, ru, rd, bias, bias + 16, dg, du, h);
                     else if (a.act == kActGelu) grad_cols<T, kActGelu>(rg, ru, rd, bias, bias + 16, dg, du, h);
                     else grad_cols<T, kActRelu>(rg, ru, rd, bias, bias + 16, dg, du, h);
-                    // room in p: dx of the step before has read it, and so have the stores (all four warps'
-                    // of these rows; at a tile's start, every warp's staging of the tile before)
+                    // room in p: dx of the step before and the stores have read it; at a tile's start, every
+                    // warp's staging of the tile before too
                     mbar_wait_w(&bars->p_empty, (i & 1) ^ 1, abort);
+                    mbar_wait_w(&bars->p_read, (i & 1) ^ 1, abort);
                     if (c == 0) {
                         if (lane == 0) tma_store_wait_read<0>();
                         __syncwarp();
                         named_bar_sync(5, 32 * kEpiWarps);
-                    } else {
-                        if (part == 0 && lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-                        named_bar_sync(1 + quad, 128);
                     }
                     const uint32_t o0 = sw128_off(prow, part * 2), o1 = sw128_off(prow, part * 2 + 1);
                     *reinterpret_cast<uint4*>(p + o0) = pack8<T>(dg);
@@ -385,41 +389,40 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                     *reinterpret_cast<uint4*>(p + 2 * kTile + o1) = make_uint4(h[4], h[5], h[6], h[7]);
                     fence_async_shared();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_pair(p_full);
-                    named_bar_sync(1 + quad, 128);
-                    if (part == 0 && lane == 0 && row < a.rows) {
-                        const uint32_t src = smem_u32(s_p + quad * 4096);
-#pragma unroll
-                        for (int s = 0; s < 3; ++s) tma_store_3d(&maps.p, src + s * kTile, c * 64, row, s);
-                        tma_store_commit();
+                    if (lane == 0) {
+                        mbar_arrive_pair(p_full);
+                        mbar_arrive(&bars->p_quad[quad]);
                     }
-                    // one warp adds to an address, in the order of its steps: the same bits every time
-                    const float sg = column_sum(dg, lane), su = column_sum(du, lane);
-                    const int cs = col + (lane >> 1);
-                    if (cs < a.hidden) atomicAdd(sums + (lane & 1 ? a.hidden : 0) + cs, lane & 1 ? su : sg);
+                    // column sums of what was written (this warp's own rows and columns); one warp adds to an
+                    // address, in the order of its steps: the same bits every time
+                    const float2 sg = tile_column_sums<T>(smem_u32(s_p), quad * 32, part * 2, lane);
+                    const float2 su = tile_column_sums<T>(smem_u32(s_p) + kTile, quad * 32, part * 2, lane);
+                    const float v = lane & 2 ? (lane & 1 ? su.y : su.x) : (lane & 1 ? sg.y : sg.x);
+                    const int cs = col + (lane & 1) * 8 + (lane >> 2);
+                    if (cs < a.hidden) atomicAdd(sums + (lane & 2 ? a.hidden : 0) + cs, v);
                 }
             }
             // ---- the tile's output: 64 columns a warp (32 where bn is 128)
             const int cols = a.bn / 4, col0 = part * cols;
-            uint4 res[8];
+            // Residual rows, 32 columns at a time: four lanes a row (a thread on a row of its own would touch 32
+            // lines an instruction: 128 such instructions took 4000 cycles), in flight while the last products run;
+            // they reach the row's thread through the staging buffer.
+            uint4 res[4];
             float down[2] = {0.0f, 0.0f};
+            auto load_res = [&](int g) {
+                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + (lane >> 2)) * a.residual_stride + col0 + g + 8 * (lane & 3);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)  // dim is a multiple of 8: a group is inside or outside
+                    res[q] = row + (lane >> 2) + 8 * q < a.rows && col0 + g + 8 * (lane & 3) < a.dim
+                                 ? *reinterpret_cast<const uint4*>(r + 8 * q * a.residual_stride) : make_uint4(0, 0, 0, 0);
+            };
             if (!BWD) {
                 down[0] = ld_bias<T>(a.b_down, col0 + lane, a.dim);
                 if (cols > 32) down[1] = ld_bias<T>(a.b_down, col0 + 32 + lane, a.dim);
-            }
-            if (!BWD && a.residual) {  // in flight while the last products run
-                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + lane) * a.residual_stride + col0;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)  // dim is a multiple of 8: a group is inside or outside
-                    res[q] = row + lane < a.rows && 8 * q < cols && col0 + 8 * q < a.dim ? *reinterpret_cast<const uint4*>(r + 8 * q)
-                                                                                          : make_uint4(0, 0, 0, 0);
+                if (a.residual) load_res(0);
             }
             mbar_wait_w(&bars->o_full, it & 1, abort);
-            if (BWD) {  // p becomes staging: its last products are done, and its last stores have been read
-                if (lane == 0) tma_store_wait_read<0>();
-                __syncwarp();
-                named_bar_sync(5, 32 * kEpiWarps);
-            }
+            if (BWD) mbar_wait_w(&bars->p_read, (i & 1) ^ 1, abort);  // p becomes staging: its last stores have read it
             tc_fence_after();
 #pragma unroll
             for (int g = 0; g < 64; g += 32) {
@@ -440,9 +443,16 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                             r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, down[g / 32], j));
                     }
                     if (a.residual) {
+                        if (lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *reinterpret_cast<uint4*>(buf + sw64_off((lane >> 2) + 8 * q, lane & 3)) = res[q];
+                        __syncwarp();
+                        if (g + 32 < cols) load_res(g + 32);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const uint4 v = res[g / 8 + q];
+                            const uint4 v = *reinterpret_cast<const uint4*>(buf + sw64_off(lane, q));
                             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
@@ -484,7 +494,7 @@ cudaError_t launch(const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStr
     auto k = gated_fused_kernel<T, BWD>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BWD>::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k, dim3(2 * fused_pairs(a.tiles, sm_count)), dim3(kThreads), Cfg<BWD>::kSmem, s, a, m);
+    return launch_pdl(k, dim3(2 * fused_pairs(a.tiles, sm_count)), dim3(Cfg<BWD>::kThreads), Cfg<BWD>::kSmem, s, a, m);
 }
 
 }  // namespace
