@@ -687,9 +687,10 @@ int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated
         FusedMaps m;
         fused_args(ctx, p, w, rows, a);
         a.b_down = w->b_down;
-        a.residual = residual ? static_cast<const T*>(residual) + r0 * rs : nullptr;
-        a.residual_stride = rs;
-        if ((rc = fused_maps(p, w, static_cast<const T*>(x) + r0 * xs, xs, rows, 128, m)) ||
+        a.residual = residual != nullptr;
+        if ((rc = residual ? make_map(&m.residual, static_cast<const T*>(residual) + r0 * rs, p->dtype, p->dim, rows, 0, rs, 32, 32, kSw64)
+                           : PRISM_OK) ||
+            (rc = fused_maps(p, w, static_cast<const T*>(x) + r0 * xs, xs, rows, 128, m)) ||
             (rc = make_map(&m.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 64, a.bn / 2, kSw128)) ||
             (rc = make_map(&m.out, static_cast<T*>(y) + r0 * ys, p->dtype, p->dim, rows, 0, ys, 32, 32, kSw64)) ||
             (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, false, a, m, ctx->sm_count, s), who)))

@@ -23,22 +23,26 @@ constexpr int kTile = 16384;   // 128 rows x 64 columns
 
 template <bool BWD>
 struct Cfg {
-    // producer, MMA issuer, epilogue warps; backward, a last one that stores p
-    static constexpr int kThreads = 32 * (2 + kEpiWarps + BWD);
+    // Producer, MMA issuer, epilogue warps; then, backward, one that stores p; forward, four that write the
+    // output while the epilogue warps, bound by their exponentials and reciprocals, go on with the next tile.
+    static constexpr int kThreads = 32 * (2 + kEpiWarps + (BWD ? 1 : 4));
     static constexpr int kStep = BWD ? 64 : 128;  // hidden columns a step
     static constexpr int kCols = kStep / 4;       // of an epilogue warp
     static constexpr int kRing = 3, kStage = BWD ? 16384 : 32768;
     static constexpr int kXBytes = (BWD ? 8 : 4) * kTile;  // x, dy: four K-blocks each
     static constexpr int kPBytes = (BWD ? 3 : 2) * kTile;  // dg, du, h, or h
-    static constexpr int kBias = 2 * kCols * 4;  // bytes a warp
+    static constexpr int kOut = BWD ? 0 : 4 * 3 * 2048;  // forward: three 32 x 32 boxes an output warp (backward: in p)
+    static constexpr int kDown = BWD ? 0 : 1024;         // the output's bias
+    static constexpr int kBias = 2 * kCols * 4;          // bytes an epilogue warp
     // the dynamic shared memory of a kernel without static shared memory starts 1024-byte aligned
-    static constexpr int kSmem = kXBytes + kPBytes + kRing * kStage + kEpiWarps * kBias + 512;
+    static constexpr int kSmem = kXBytes + kPBytes + kRing * kStage + kOut + kDown + kEpiWarps * kBias + 512;
     static_assert(kSmem <= 232448, "227 KB");
     static constexpr int kAcc = 256;  // first TMEM column of [g | u (| dh)], behind the output accumulator
 };
 struct Bars {
     uint64_t full[3], empty[3], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
     uint64_t p_quad[4], p_read;  // backward: a quad's rows of p are written; p's stores have read it
+    uint64_t res_full[4][3];     // forward: a box of the residual has landed
     uint32_t tmem_base;
     int abort;
 };
@@ -46,6 +50,13 @@ struct Bars {
 template <typename T>
 PRISM_DEV float ld_bias(const void* b, int i, int n) {
     return b && i < n ? to_f32(static_cast<const T*>(b)[i]) : 0.0f;
+}
+
+// A 32 x 32 box of a warp's rows: this lane's row as 16 packed pairs into 64-byte swizzled rows.
+PRISM_DEV void stage_row64(unsigned char* buf, int lane, const uint32_t (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
 
 template <typename T, int ACT>
@@ -73,7 +84,9 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
     unsigned char* s_x = smem;
     unsigned char* s_p = s_x + C::kXBytes;
     unsigned char* s_ring = s_p + C::kPBytes;
-    unsigned char* s_bias = s_ring + C::kRing * C::kStage;
+    unsigned char* s_out = s_ring + C::kRing * C::kStage;
+    float* s_down = reinterpret_cast<float*>(s_out + C::kOut);
+    unsigned char* s_bias = s_out + C::kOut + C::kDown;
     Bars* bars = reinterpret_cast<Bars*>(s_bias + kEpiWarps * C::kBias);
     volatile int* abort = &bars->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -95,7 +108,8 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         mbar_init(&bars->p_full, 2 * kEpiWarps);
         mbar_init(&bars->p_empty, 1);
         mbar_init(&bars->o_full, 1);
-        mbar_init(&bars->o_empty, 2 * kEpiWarps);
+        mbar_init(&bars->o_empty, 2 * (BWD ? kEpiWarps : 4));
+        for (int q = 0; q < 12; ++q) mbar_init(&bars->res_full[0][q], 1);
         for (int q = 0; q < 4; ++q) mbar_init(&bars->p_quad[q], 4);
         mbar_init(&bars->p_read, 1);
         bars->abort = (smem_u32(smem) & 1023u) != 0;
@@ -261,12 +275,80 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                 __syncwarp();
             }
         if (lane == 0) tma_store_wait0();
+    } else if (!BWD && warp >= 2 + kEpiWarps) {
+        // ---- output (forward): 32 rows a warp, 32 columns at a time.  The residual's boxes come by TMA two ahead
+        // into the staging buffers that the output leaves from (a thread that reads a row of its own from
+        // global memory touches 32 lines an instruction: 4000 cycles a tile).
+        const int quad = warp & 3;
+        unsigned char* bufs = s_out + quad * 3 * 2048;
+        const uint32_t o_empty = peer_addr(smem_u32(&bars->o_empty), 0);
+        for (int j = threadIdx.x - 32 * (2 + kEpiWarps); j < 256; j += 128) s_down[j] = ld_bias<T>(a.b_down, j, a.dim);
+        named_bar_sync(6, 128);
+        const int boxes = (a.dim + 31) / 32;
+        uint32_t it = 0, n = 0;  // n: boxes so far
+        for (int tile = pair; tile < a.tiles; tile += pairs, ++it) {
+            const int row = tile * 256 + rank * 128 + quad * 32;
+            auto load_res = [&](int box) {
+                const uint32_t k = (n + box) % 3;
+                if (a.residual && box < boxes && lane == 0) {
+                    mbar_expect_tx(&bars->res_full[quad][k], 2048);
+                    tma_load_2d(smem_u32(bufs + k * 2048), &maps.residual, &bars->res_full[quad][k], box * 32, row);
+                }
+            };
+            if (lane == 0) tma_store_wait_read<0>();
+            load_res(0);
+            load_res(1);
+            mbar_wait_step(&bars->o_full, it & 1, abort);
+            tc_fence_after();
+            for (int g = 0; g < boxes; ++g) {
+                const uint32_t k = (n + g) % 3;
+                unsigned char* buf = bufs + k * 2048;
+                uint32_t r[32], o[16];
+                tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + g * 32, r);
+                if (a.residual) mbar_wait_step(&bars->res_full[quad][k], ((n + g) / 3) & 1, abort);
+                tmem_ld_wait();
+                if (g == boxes - 1) {  // all read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(o_empty);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint4 v = a.residual ? *reinterpret_cast<const uint4*>(buf + sw64_off(lane, q)) : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float f0, f1, y0, y1;
+                        unpack2<T>(w[j], f0, f1);
+                        const int i = 8 * q + 2 * j;
+                        const uint64_t bias = *reinterpret_cast<const uint64_t*>(s_down + g * 32 + i);
+                        f2_unpack(f2_add(f2_add(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), bias), f2_pack(f0, f1)), y0, y1);
+                        o[4 * q + j] = pack2<T>(y0, y1);
+                    }
+                }
+                if (!a.residual) {  // with one, the loads have waited for the buffer's last store
+                    if (lane == 0) tma_store_wait_read<2>();
+                    __syncwarp();
+                }
+                stage_row64(buf, lane, o);
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    if (row < a.rows) tma_store_2d(&maps.out, smem_u32(buf), g * 32, row);
+                    tma_store_commit();
+                    if (a.residual) tma_store_wait_read<1>();  // the box before: its buffer is the next load's
+                }
+                load_res(g + 2);
+            }
+            n += boxes;
+        }
+        if (lane == 0) tma_store_wait0();
     } else {
         // ---- epilogue
         constexpr int kBiasVals = C::kBias / 128;
         const int quad = warp & 3, part = (warp - 2) >> 2;
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-        unsigned char* buf = s_p + (warp - 2) * 2048;  // store staging, once the tile's steps are done
+        unsigned char* buf = s_p + (warp - 2) * 2048;  // backward: store staging, once the tile's steps are done
         float* bias = reinterpret_cast<float*>(s_bias + (warp - 2) * C::kBias);
         const uint32_t acc_empty = peer_addr(smem_u32(&bars->acc_empty), 0), o_empty = peer_addr(smem_u32(&bars->o_empty), 0);
         const uint32_t p_full = peer_addr(smem_u32(&bars->p_full), 0);
@@ -295,10 +377,6 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         uint32_t it = 0, i = 0;
         for (int tile = pair; tile < a.tiles; tile += pairs, ++it) {
             const int row = tile * 256 + rank * 128 + quad * 32;
-            if (!BWD && a.residual && row + lane < a.rows && part * a.bn / 4 < a.dim) {  // on its way to L2: this warp's columns, a line at most
-                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + lane) * a.residual_stride + part * a.bn / 4;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(r));
-            }
             if (BWD) {  // dy's column sums, while the first products run: 64 columns a warp
                 const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
                 for (int c = part * 64; c < min(a.dim, part * 64 + 64); c += 32) {
@@ -344,11 +422,6 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     else if (a.act == kActGelu) gate32<T, kActGelu>(rg, ru, bias, bias + 32, h);
                     else gate32<T, kActRelu>(rg, ru, bias, bias + 32, h);
                     mbar_wait_w(&bars->p_empty, (i & 1) ^ 1, abort);  // y of the step before has read p
-                    if (c == 0) {  // and the stores of the tile before
-                        if (lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-                        named_bar_sync(5, 32 * kEpiWarps);
-                    }
                     unsigned char* p = s_p + (part >> 1) * kTile;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -402,27 +475,11 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     if (cs < a.hidden) atomicAdd(sums + (lane & 2 ? a.hidden : 0) + cs, v);
                 }
             }
-            // ---- the tile's output: 64 columns a warp (32 where bn is 128)
+            if (!BWD) continue;
+            // ---- the tile's dx: 64 columns a warp (32 where bn is 128)
             const int cols = a.bn / 4, col0 = part * cols;
-            // Residual rows, 32 columns at a time: four lanes a row (a thread on a row of its own would touch 32
-            // lines an instruction: 128 such instructions took 4000 cycles), in flight while the last products run;
-            // they reach the row's thread through the staging buffer.
-            uint4 res[4];
-            float down[2] = {0.0f, 0.0f};
-            auto load_res = [&](int g) {
-                const T* r = static_cast<const T*>(a.residual) + (int64_t)(row + (lane >> 2)) * a.residual_stride + col0 + g + 8 * (lane & 3);
-#pragma unroll
-                for (int q = 0; q < 4; ++q)  // dim is a multiple of 8: a group is inside or outside
-                    res[q] = row + (lane >> 2) + 8 * q < a.rows && col0 + g + 8 * (lane & 3) < a.dim
-                                 ? *reinterpret_cast<const uint4*>(r + 8 * q * a.residual_stride) : make_uint4(0, 0, 0, 0);
-            };
-            if (!BWD) {
-                down[0] = ld_bias<T>(a.b_down, col0 + lane, a.dim);
-                if (cols > 32) down[1] = ld_bias<T>(a.b_down, col0 + 32 + lane, a.dim);
-                if (a.residual) load_res(0);
-            }
             mbar_wait_w(&bars->o_full, it & 1, abort);
-            if (BWD) mbar_wait_w(&bars->p_read, (i & 1) ^ 1, abort);  // p becomes staging: its last stores have read it
+            mbar_wait_w(&bars->p_read, (i & 1) ^ 1, abort);  // p becomes staging: its last stores have read it
             tc_fence_after();
 #pragma unroll
             for (int g = 0; g < 64; g += 32) {
@@ -435,47 +492,15 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     __syncwarp();
                     if (lane == 0) mbar_arrive_pair(o_empty);
                 }
-                const int c = col0 + g;
-                if (!BWD) {
-                    if (a.b_down) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, down[g / 32], j));
-                    }
-                    if (a.residual) {
-                        if (lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            *reinterpret_cast<uint4*>(buf + sw64_off((lane >> 2) + 8 * q, lane & 3)) = res[q];
-                        __syncwarp();
-                        if (g + 32 < cols) load_res(g + 32);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(buf + sw64_off(lane, q));
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                float f0, f1;
-                                unpack2<T>(w[j], f0, f1);
-                                const int k = 8 * q + 2 * j;
-                                r[k] = __float_as_uint(__uint_as_float(r[k]) + f0);
-                                r[k + 1] = __float_as_uint(__uint_as_float(r[k + 1]) + f1);
-                            }
-                        }
-                    }
-                }
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
                 if (lane == 0) tma_store_wait_read<0>();
                 __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                stage_row64(buf, lane, o);
                 fence_async_shared();
                 __syncwarp();
-                if (lane == 0 && c < a.dim && row < a.rows) {
-                    tma_store_2d(&maps.out, smem_u32(buf), c, row);
+                if (lane == 0 && col0 + g < a.dim && row < a.rows) {
+                    tma_store_2d(&maps.out, smem_u32(buf), col0 + g, row);
                     tma_store_commit();
                 }
             }

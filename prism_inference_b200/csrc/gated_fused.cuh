@@ -11,6 +11,7 @@ constexpr int kFusedMaxDim = 256;
 // forward, {64, 64} backward; the others by direction.
 struct FusedMaps {
     CUtensorMap x, wg, wu, out;  // out: y or dx, box {32, 32}
+    CUtensorMap residual;        // forward, where there is one: box {32, 32}
     CUtensorMap wd;              // forward: [dim][hidden], box {64, bn / 2}; backward: box {32, 128}, 64-byte swizzle
     CUtensorMap dy, wg_mn, wu_mn, p;  // backward: boxes {64, 64} of the weights; p [3][rows][hidden], box {64, 32}
 };
@@ -21,8 +22,7 @@ struct FusedArgs {
     int act;
     int first;   // backward: the first chunk of rows, column sums start here
     const void *b_gate, *b_up, *b_down;
-    const void* residual;
-    int64_t residual_stride;
+    int residual;  // forward: there is one
     float *sums, *sums_dy;  // backward: [CTAs][4][2 hidden] and [CTAs][4][dim]
     const void* dy;
     int64_t dy_stride;
