@@ -324,8 +324,9 @@ int prism_gated_ffn(prism_ctx* ctx, const prism_gated_params* p, const prism_gat
 int prism_gated_ffn_backward(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
                              const void* dy, void* dx, const prism_gated_grads* grads, void* workspace,
                              size_t workspace_bytes, void* stream);
-/* The workspace of the forward (backward = 0) or backward (1) call: bounded, it does not grow with
- * rows beyond some ten thousand. */
+/* The workspace of the forward (backward = 0) or backward (1) call.  Forward: none for dim <= 256, else
+ * 2 hidden bytes a row up to 1 GiB (rows go through in chunks).  Backward: 6 hidden bytes a row up to
+ * 1 GiB, and fp32 partial sums of the gradients. */
 int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_params* p, int backward, size_t* bytes);
 
 /* ---- fast path: a whole stack over a batch of frames ------------------------ */

@@ -13,7 +13,7 @@
 //   DOWN  y = h Wd^T
 //   BACK  dh = dy Wd and [g | u] again from x -> dg, du, h, and the bias gradients' sums on the way
 //   XW    dx tiles and dW tiles (split over rows) in one launch: neither fills the GPU alone
-// Rows go through in chunks, so the scratch memory does not grow with the batch.
+// Rows go through in chunks, so the scratch memory stays bounded.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -592,8 +592,14 @@ int launch(const prism_ctx* ctx, const Args& a, const Maps& m, cudaStream_t s, c
     return cuda_rc(launch_pdl(k, dim3(2 * pairs), dim3(Cfg<KIND>::kThreads), Cfg<KIND>::kSmem, s, a, m), who);
 }
 
-// Rows that go through at a time: a row tile for every CTA pair.
-int64_t chunk_rows(const prism_ctx* ctx, int64_t rows) { return std::min<int64_t>(rows, (int64_t)(ctx->sm_count / 2) * 256); }
+// Rows that go through at a time: whole waves of a row tile for every CTA pair, as many as keep
+// `row_bytes` of scratch a row within 1 GiB, one at least.  (130,560 x 256, hidden 1024, backward: 635 us
+// by single waves, whose scratch half stays in L2, 559 us in one piece: launches and their first
+// loads cost more than L2 gives.)
+int64_t chunk_rows(const prism_ctx* ctx, int64_t rows, int64_t row_bytes) {
+    const int64_t wave = (int64_t)(ctx->sm_count / 2) * 256;
+    return std::min<int64_t>(rows, wave * std::max<int64_t>(1, (1ll << 30) / row_bytes / wave));
+}
 
 inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
@@ -607,7 +613,7 @@ struct BackPlan {
 };
 BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     BackPlan b;
-    b.chunk = chunk_rows(ctx, p->rows);
+    b.chunk = chunk_rows(ctx, p->rows, 6 * (int64_t)p->hidden);
     const int bn = p->dim <= 128 ? 128 : 256;
     const int64_t tiles = 3 * ((p->hidden + 255) / 256) * (int64_t)((p->dim + bn - 1) / bn);
     const int64_t kb = (b.chunk + 63) / 64;
@@ -697,7 +703,7 @@ int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated
             return rc;
     }
     if (p->dim <= kFusedMaxDim) return PRISM_OK;
-    const int64_t chunk = chunk_rows(ctx, p->rows);
+    const int64_t chunk = chunk_rows(ctx, p->rows, 2 * (int64_t)p->hidden);
     for (int64_t r0 = 0; r0 < p->rows; r0 += chunk) {
         const int rows = (int)std::min(chunk, p->rows - r0);
         const T* xc = static_cast<const T*>(x) + r0 * xs;
@@ -834,9 +840,9 @@ extern "C" int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_param
     if (!ctx || !p || !bytes) return fail(PRISM_E_ARG, "prism_gated_ffn_workspace: NULL argument");
     int rc = check_gated("prism_gated_ffn_workspace", p);
     if (rc) return rc;
-    *bytes = p->rows == 0                                    ? 0
-             : backward                                    ? back_plan(ctx, p).total()
-             : p->dim <= kFusedMaxDim ? 0 : (size_t)chunk_rows(ctx, p->rows) * p->hidden * 2;
+    *bytes = p->rows == 0 ? 0
+             : backward   ? back_plan(ctx, p).total()
+             : p->dim <= kFusedMaxDim ? 0 : (size_t)chunk_rows(ctx, p->rows, 2 * (int64_t)p->hidden) * p->hidden * 2;
     return PRISM_OK;
 }
 
