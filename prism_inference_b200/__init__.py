@@ -17,6 +17,7 @@ No entry point falls back to the CPU: a missing libprism_moe.so raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 from . import abi, configs, layout, synth
 from .abi import (AttnParams, DenseParams, DropoutParams, ExpertParams, GatedGrads, GatedParams, GatedWeights, NormParams,
@@ -55,55 +56,82 @@ _DTYPES = {}  # torch dtype -> prism_dtype
 
 
 def _dtype(t, name: str) -> int:
-    if not _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         import torch
         _DTYPES.update({getattr(torch, d): i for i, d in enumerate(abi.DTYPES)})
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"{name}: dtype {t.dtype} (fp16, bf16 or fp32)") from None
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"{name}: dtype {t.dtype} (fp16, bf16 or fp32)")
+        code = _DTYPES[t.dtype]
+    return code
 
 
-def _rows(t, name: str, like=None):
-    """(rows, dim, row stride) of a tensor [..., dim] whose last dimension is consecutive in memory;
-    `like` = (tensor, rows, dim) it must match in type, device, rows and dim."""
-    if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+@functools.lru_cache(None)
+def _F32():
+    import torch
+    return torch.float32
+
+
+@functools.lru_cache(None)
+def _raw_stream():
+    """device -> handle of torch's current stream (torch.cuda.current_stream makes an object for it)."""
+    import torch
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+@functools.lru_cache(None)
+def _I64():
+    import torch
+    return torch.int64
+
+
+# These run on every call of the operators below, whose smallest calls take less time than their
+# checks: few attribute look-ups (a tensor's shape, device and so on are objects made anew each time).
+def _rows(t, name: str):
+    """(rows, dim, row stride) of a tensor [..., dim] whose last dimension is consecutive in memory."""
+    shape = t.shape
+    if len(shape) == 2:
+        rows, dim = shape
+        stride, last = t.stride()
+        if last != 1 and dim > 1:
+            raise ValueError(f"{name}: the last dimension is not consecutive in memory")
+        return rows, dim, stride if rows > 1 else dim
+    if len(shape) < 1 or (shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name}: the last dimension is not consecutive in memory")
-    dim = t.shape[-1]
-    if t.dim() == 2:
-        rows, stride = t.shape[0], t.stride(0)
-    else:
-        rows, stride = t.numel() // max(1, dim), dim
-        if not t.is_contiguous():
-            try:
-                stride = t.view(-1, dim).stride(0)
-            except RuntimeError:
-                raise ValueError(f"{name}: its rows do not lie at one stride") from None
-    if rows <= 1:
-        stride = dim
-    if like is not None:
-        ref, r, d = like
-        if t.dtype != ref.dtype or t.device != ref.device or rows != r or dim != d:
-            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device} beside {ref.dtype} [{r}, {d}] on {ref.device}")
-    return rows, dim, stride
+    dim = shape[-1]
+    rows, stride = t.numel() // max(1, dim), dim
+    if not t.is_contiguous():
+        try:
+            stride = t.view(-1, dim).stride(0)
+        except RuntimeError:
+            raise ValueError(f"{name}: its rows do not lie at one stride") from None
+    return rows, dim, stride if rows > 1 else dim
 
 
-def _flat(t, name: str, shape, dtype, device) -> int | None:
+def _stride(t, name: str, dtype, device: int, rows: int, dim: int) -> int:
+    """Row stride of a tensor [..., dim] that has to be of this type, device and size."""
+    r, d, stride = _rows(t, name)
+    if r != rows or d != dim or t.dtype is not dtype or t.get_device() != device:
+        raise ValueError(f"{name}: {t.dtype} {list(t.shape)} on {t.device}, expected {dtype} [{rows}, {dim}] on cuda:{device}")
+    return stride
+
+
+def _flat(t, name: str, shape, dtype, device: int) -> int | None:
     """Address of a contiguous parameter, gradient or statistics tensor; None passes through."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} "
-                         f"on {t.device}")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} {list(shape)} on cuda:{device}, got {t.dtype} "
+                         f"{list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _workspace(workspace, nbytes: int, device, stream):
+def _workspace(workspace, nbytes: int, device: int, stream):
     """(tensor, address, bytes): the caller's workspace, or one from torch's allocator that belongs to
     the call's stream (so it is not handed out again before the call's work has run)."""
     if workspace is not None:
-        if workspace.device != device or not workspace.is_contiguous():
-            raise ValueError(f"workspace: expected a contiguous tensor on {device}")
+        if workspace.get_device() != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace: expected a contiguous tensor on cuda:{device}")
         return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
     if not nbytes:
         return None, None, 0
@@ -124,6 +152,7 @@ class Prism:
     def __init__(self, device: int = 0):
         self.lib = abi.load()
         self.device = device
+        self._workspaces = {}  # bytes of scratch by call and sizes
         h = C.c_void_p()
         check(self.lib, self.lib.prism_create(device, C.byref(h)))
         self.h = h
@@ -190,110 +219,117 @@ class Prism:
     # slices of wider buffers work); the caller allocates outputs.  stream: None = torch's current
     # stream of the context's device; tensors made on another stream are the caller's to order.
     # workspace: scratch memory of at least the *_workspace() bytes, None = from torch's allocator.
-    def _on_device(self, t, name: str):
-        if not t.is_cuda or t.device.index != self.device:
-            raise ValueError(f"{name}: on {t.device}, the context is for cuda:{self.device}")
-
     def _stream(self, stream):
         if stream is None:
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return _raw_stream()(self.device)
         return getattr(stream, "cuda_stream", stream)
 
+    def _scratch(self, query, p, key, *args) -> int:
+        """Bytes of workspace that `query` answers for params p: a function of the sizes in `key`, asked once."""
+        n = self._workspaces.get(key)
+        if n is None:
+            need = C.c_size_t()
+            check(self.lib, query(self.h, C.byref(p), *args, C.byref(need)))
+            if len(self._workspaces) >= 1024:  # ragged batches: sizes that hardly come again
+                self._workspaces.clear()
+            n = self._workspaces[key] = need.value
+        return n
+
     @staticmethod
-    def _param_dtype(ps, x):
+    def _param_dtype(x, *params):
         """dtype of the norm's parameters: the first given one's (fp32 or the rows' own), else the rows'."""
-        for p in ps:
+        for p in params:
             if p is not None:
-                return p.dtype, _dtype(p, "weight")
-        return x.dtype, _dtype(x, "x")
+                return p.dtype
+        return x.dtype
 
     def layer_norm(self, x, weight, bias, y, eps: float = 1e-5, mean=None, rstd=None, stream=None):
         """prism_layer_norm: y = (x - mean) * rstd * weight + bias over the last dimension.  weight, bias
         ([dim], x's dtype or fp32) and the fp32 statistics mean, rstd ([rows]) are optional."""
-        import torch
-        self._on_device(x, "x")
-        rows, dim, xs = _rows(x, "x")
-        ys = _rows(y, "y", (x, rows, dim))[2]
-        pt, pcode = self._param_dtype((weight, bias), x)
-        p = NormParams(rows=rows, x_stride=xs, y_stride=ys, dim=dim, dtype=_dtype(x, "x"), param_dtype=pcode, eps=eps)
-        check(self.lib, self.lib.prism_layer_norm(
-            self.h, C.byref(p), _ptr(x), _flat(weight, "weight", (dim,), pt, x.device),
-            _flat(bias, "bias", (dim,), pt, x.device), _ptr(y), _flat(mean, "mean", (rows,), torch.float32, x.device),
-            _flat(rstd, "rstd", (rows,), torch.float32, x.device), self._stream(stream)))
+        dev, dt, (rows, dim, xs) = self.device, x.dtype, _rows(x, "x")
+        if x.get_device() != dev:
+            raise ValueError(f"x: on {x.device}, the context is for cuda:{dev}")
+        code, pt = _dtype(x, "x"), self._param_dtype(x, weight, bias)
+        p = NormParams(rows, xs, _stride(y, "y", dt, dev, rows, dim), 0, 0, 0, dim, code, _DTYPES.get(pt, -1), eps)
+        f32 = _F32()
+        rc = self.lib.prism_layer_norm(
+            self.h, C.byref(p), x.data_ptr(), _flat(weight, "weight", (dim,), pt, dev), _flat(bias, "bias", (dim,), pt, dev),
+            y.data_ptr(), _flat(mean, "mean", (rows,), f32, dev), _flat(rstd, "rstd", (rows,), f32, dev), self._stream(stream))
+        if rc:
+            check(self.lib, rc)
         return y
 
     def layer_norm_backward(self, x, weight, mean, rstd, dy, dx, dweight=None, dbias=None, add=None, workspace=None,
                             stream=None):
         """prism_layer_norm_backward: dx (+ add, the gradient that came past the norm), and the parameters'
         gradients where dweight, dbias are given (overwritten)."""
-        import torch
-        self._on_device(x, "x")
-        rows, dim, xs = _rows(x, "x")
-        like = (x, rows, dim)
-        pt, pcode = self._param_dtype((weight, dweight, dbias), x)
-        p = NormParams(rows=rows, x_stride=xs, dy_stride=_rows(dy, "dy", like)[2], dx_stride=_rows(dx, "dx", like)[2],
-                       add_stride=_rows(add, "add", like)[2] if add is not None else 0, dim=dim, dtype=_dtype(x, "x"),
-                       param_dtype=pcode)
-        need = C.c_size_t()
+        dev, dt, (rows, dim, xs) = self.device, x.dtype, _rows(x, "x")
+        if x.get_device() != dev:
+            raise ValueError(f"x: on {x.device}, the context is for cuda:{dev}")
+        code, pt = _dtype(x, "x"), self._param_dtype(x, weight, dweight, dbias)
+        p = NormParams(rows, xs, 0, _stride(dy, "dy", dt, dev, rows, dim),
+                       0 if add is None else _stride(add, "add", dt, dev, rows, dim), _stride(dx, "dx", dt, dev, rows, dim), dim,
+                       code, _DTYPES.get(pt, -1), 0.0)
+        need = 0
         if dweight is not None or dbias is not None:
-            check(self.lib, self.lib.prism_layer_norm_backward_workspace(self.h, C.byref(p), C.byref(need)))
-        keep, ws, ws_bytes = _workspace(workspace, need.value, x.device, stream)
-        check(self.lib, self.lib.prism_layer_norm_backward(
-            self.h, C.byref(p), _ptr(x), _flat(weight, "weight", (dim,), pt, x.device),
-            _flat(mean, "mean", (rows,), torch.float32, x.device), _flat(rstd, "rstd", (rows,), torch.float32, x.device),
-            _ptr(dy), _ptr(add) if add is not None else None, _ptr(dx),
-            _flat(dweight, "dweight", (dim,), pt, x.device), _flat(dbias, "dbias", (dim,), pt, x.device), ws, ws_bytes,
-            self._stream(stream)))
+            need = self._scratch(self.lib.prism_layer_norm_backward_workspace, p, ("norm", rows, dim, code, pt))
+        keep, ws, ws_bytes = _workspace(workspace, need, dev, stream)
+        f32 = _F32()
+        rc = self.lib.prism_layer_norm_backward(
+            self.h, C.byref(p), x.data_ptr(), _flat(weight, "weight", (dim,), pt, dev), _flat(mean, "mean", (rows,), f32, dev),
+            _flat(rstd, "rstd", (rows,), f32, dev), dy.data_ptr(), None if add is None else add.data_ptr(), dx.data_ptr(),
+            _flat(dweight, "dweight", (dim,), pt, dev), _flat(dbias, "dbias", (dim,), pt, dev), ws, ws_bytes,
+            self._stream(stream))
+        if rc:
+            check(self.lib, rc)
         return dx
 
     def dropout_add(self, x, residual, y, p: float, rng, stream=None):
         """prism_dropout_add: y = residual + dropout(x) (residual None: dropout(x)), dropping with probability
         round(65536 p) / 65536.  rng: CUDA int64 [2] {seed, offset}, read when the call runs.  The gradient:
         the same call on it, with the same p and rng and no residual."""
-        import torch
-        self._on_device(x, "x")
-        rows, dim, xs = _rows(x, "x")
-        like = (x, rows, dim)
-        q = DropoutParams(rows=rows, x_stride=xs, y_stride=_rows(y, "y", like)[2],
-                          residual_stride=_rows(residual, "residual", like)[2] if residual is not None else 0, dim=dim,
-                          dtype=_dtype(x, "x"), threshold=max(-1, min(65536, int(round(65536 * p)))))
-        check(self.lib, self.lib.prism_dropout_add(
-            self.h, C.byref(q), _ptr(x), _ptr(residual) if residual is not None else None,
-            _flat(rng, "rng", (2,), torch.int64, x.device), _ptr(y), self._stream(stream)))
+        dev, dt, (rows, dim, xs) = self.device, x.dtype, _rows(x, "x")
+        if x.get_device() != dev:
+            raise ValueError(f"x: on {x.device}, the context is for cuda:{dev}")
+        rs = 0 if residual is None else _stride(residual, "residual", dt, dev, rows, dim)
+        q = DropoutParams(rows, xs, rs, _stride(y, "y", dt, dev, rows, dim), dim, _dtype(x, "x"),
+                          max(-1, min(65536, int(round(65536 * p)))))
+        rc = self.lib.prism_dropout_add(self.h, C.byref(q), x.data_ptr(), None if residual is None else residual.data_ptr(),
+                                        _flat(rng, "rng", (2,), _I64(), dev), y.data_ptr(), self._stream(stream))
+        if rc:
+            check(self.lib, rc)
         return y
 
     def _gated(self, x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
-        """(params, weights, rows, dim, hidden) of a gated feed-forward call."""
-        self._on_device(x, "x")
-        rows, dim, xs = _rows(x, "x")
-        hidden, dt, dev = w_gate.shape[0], x.dtype, x.device
+        """(params, weights, dtype, rows, dim, hidden) of a gated feed-forward call."""
+        dev, dt, (rows, dim, xs) = self.device, x.dtype, _rows(x, "x")
+        if x.get_device() != dev:
+            raise ValueError(f"x: on {x.device}, the context is for cuda:{dev}")
         if activation not in abi.ACTIVATIONS:
             raise ValueError(f"activation {activation!r}: one of {', '.join(abi.ACTIVATIONS)}")
+        hidden = w_gate.shape[0]
         w = GatedWeights(_flat(w_gate, "w_gate", (hidden, dim), dt, dev), _flat(b_gate, "b_gate", (hidden,), dt, dev),
                          _flat(w_up, "w_up", (hidden, dim), dt, dev), _flat(b_up, "b_up", (hidden,), dt, dev),
                          _flat(w_down, "w_down", (dim, hidden), dt, dev), _flat(b_down, "b_down", (dim,), dt, dev))
-        p = GatedParams(rows=rows, x_stride=xs, dim=dim, hidden=hidden, dtype=_dtype(x, "x"),
-                        activation=abi.ACTIVATIONS.index(activation))
-        return p, w, rows, dim, hidden
-
-    def _gated_workspace(self, p, backward: int, workspace, device, stream):
-        need = C.c_size_t()
-        check(self.lib, self.lib.prism_gated_ffn_workspace(self.h, C.byref(p), backward, C.byref(need)))
-        return _workspace(workspace, need.value, device, stream)
+        p = GatedParams(rows, xs, 0, 0, 0, 0, dim, hidden, _dtype(x, "x"), abi.ACTIVATIONS.index(activation))
+        return p, w, dt, rows, dim, hidden
 
     def gated_ffn(self, x, w_gate, w_up, w_down, y, b_gate=None, b_up=None, b_down=None, residual=None,
                   activation: str = "gelu", workspace=None, stream=None):
         """prism_gated_ffn: y = w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down + residual, fp16 or
         bf16; activation "gelu" (tanh form), "silu" or "relu"."""
-        p, w, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-        p.y_stride = _rows(y, "y", (x, rows, dim))[2]
+        p, w, dt, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
+        dev = self.device
+        p.y_stride = _stride(y, "y", dt, dev, rows, dim)
         if residual is not None:
-            p.residual_stride = _rows(residual, "residual", (x, rows, dim))[2]
-        keep, ws, ws_bytes = self._gated_workspace(p, 0, workspace, x.device, stream)
-        check(self.lib, self.lib.prism_gated_ffn(self.h, C.byref(p), C.byref(w), _ptr(x),
-                                                 _ptr(residual) if residual is not None else None, _ptr(y), ws, ws_bytes,
-                                                 self._stream(stream)))
+            p.residual_stride = _stride(residual, "residual", dt, dev, rows, dim)
+        need = self._scratch(self.lib.prism_gated_ffn_workspace, p, ("gated", rows, dim, hidden, p.dtype), 0)
+        keep, ws, ws_bytes = _workspace(workspace, need, dev, stream)
+        rc = self.lib.prism_gated_ffn(self.h, C.byref(p), C.byref(w), x.data_ptr(),
+                                      None if residual is None else residual.data_ptr(), y.data_ptr(), ws, ws_bytes,
+                                      self._stream(stream))
+        if rc:
+            check(self.lib, rc)
         return y
 
     def gated_ffn_backward(self, x, w_gate, w_up, w_down, dy, dx, dw_gate=None, dw_up=None, dw_down=None, b_gate=None,
@@ -301,15 +337,18 @@ class Prism:
                            stream=None):
         """prism_gated_ffn_backward: dx and the parameters' gradients that are given (overwritten), from x, the
         weights and dy; the forward pass has nothing to keep.  The residual's gradient is dy itself."""
-        p, w, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, None, activation)
-        like, dt, dev = (x, rows, dim), x.dtype, x.device
-        p.dy_stride, p.dx_stride = _rows(dy, "dy", like)[2], _rows(dx, "dx", like)[2]
+        p, w, dt, rows, dim, hidden = self._gated(x, w_gate, w_up, w_down, b_gate, b_up, None, activation)
+        dev = self.device
+        p.dy_stride, p.dx_stride = _stride(dy, "dy", dt, dev, rows, dim), _stride(dx, "dx", dt, dev, rows, dim)
         d = GatedGrads(_flat(dw_gate, "dw_gate", (hidden, dim), dt, dev), _flat(db_gate, "db_gate", (hidden,), dt, dev),
                        _flat(dw_up, "dw_up", (hidden, dim), dt, dev), _flat(db_up, "db_up", (hidden,), dt, dev),
                        _flat(dw_down, "dw_down", (dim, hidden), dt, dev), _flat(db_down, "db_down", (dim,), dt, dev))
-        keep, ws, ws_bytes = self._gated_workspace(p, 1, workspace, dev, stream)
-        check(self.lib, self.lib.prism_gated_ffn_backward(self.h, C.byref(p), C.byref(w), _ptr(x), _ptr(dy), _ptr(dx),
-                                                          C.byref(d), ws, ws_bytes, self._stream(stream)))
+        need = self._scratch(self.lib.prism_gated_ffn_workspace, p, ("gated back", rows, dim, hidden, p.dtype), 1)
+        keep, ws, ws_bytes = _workspace(workspace, need, dev, stream)
+        rc = self.lib.prism_gated_ffn_backward(self.h, C.byref(p), C.byref(w), x.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+                                               C.byref(d), ws, ws_bytes, self._stream(stream))
+        if rc:
+            check(self.lib, rc)
         return dx
 
     def status(self, stream=None):

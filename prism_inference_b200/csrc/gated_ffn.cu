@@ -586,7 +586,8 @@ constexpr CUtensorMapSwizzle kSw128 = CU_TENSOR_MAP_SWIZZLE_128B, kSw64 = CU_TEN
 template <typename T, int KIND>
 int launch(const prism_ctx* ctx, const Args& a, const Maps& m, cudaStream_t s, const char* who) {
     auto k = gated_kernel<T, KIND>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<KIND>::kSmem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(k, Cfg<KIND>::kSmem, ctx->device, done);
     if (e != cudaSuccess) return cuda_rc(e, who);
     const int pairs = std::min(a.units, ctx->sm_count / 2);
     return cuda_rc(launch_pdl(k, dim3(2 * pairs), dim3(Cfg<KIND>::kThreads), Cfg<KIND>::kSmem, s, a, m), who);
@@ -699,7 +700,7 @@ int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated
             (rc = fused_maps(p, w, static_cast<const T*>(x) + r0 * xs, xs, rows, 128, m)) ||
             (rc = make_map(&m.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 64, a.bn / 2, kSw128)) ||
             (rc = make_map(&m.out, static_cast<T*>(y) + r0 * ys, p->dtype, p->dim, rows, 0, ys, 32, 32, kSw64)) ||
-            (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, false, a, m, ctx->sm_count, s), who)))
+            (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, false, a, m, ctx, s), who)))
             return rc;
     }
     if (p->dim <= kFusedMaxDim) return PRISM_OK;
@@ -792,7 +793,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
                 (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
                 (rc = make_map(&fm.p, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 32, kSw128)) ||
                 (rc = make_map(&fm.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
-                (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx->sm_count, s), who)))
+                (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx, s), who)))
                 return rc;
             a.sums_dy = nullptr;
         } else {

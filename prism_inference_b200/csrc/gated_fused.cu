@@ -515,18 +515,19 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
 }
 
 template <typename T, bool BWD>
-cudaError_t launch(const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStream_t s) {
+cudaError_t launch(const FusedArgs& a, const FusedMaps& m, const prism_ctx* ctx, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
     auto k = gated_fused_kernel<T, BWD>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BWD>::kSmem);
+    cudaError_t e = allow_smem(k, Cfg<BWD>::kSmem, ctx->device, done);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k, dim3(2 * fused_pairs(a.tiles, sm_count)), dim3(Cfg<BWD>::kThreads), Cfg<BWD>::kSmem, s, a, m);
+    return launch_pdl(k, dim3(2 * fused_pairs(a.tiles, ctx->sm_count)), dim3(Cfg<BWD>::kThreads), Cfg<BWD>::kSmem, s, a, m);
 }
 
 }  // namespace
 
-cudaError_t launch_gated_fused(bool bf16, bool backward, const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStream_t s) {
-    if (bf16) return backward ? launch<__nv_bfloat16, true>(a, m, sm_count, s) : launch<__nv_bfloat16, false>(a, m, sm_count, s);
-    return backward ? launch<__half, true>(a, m, sm_count, s) : launch<__half, false>(a, m, sm_count, s);
+cudaError_t launch_gated_fused(bool bf16, bool backward, const FusedArgs& a, const FusedMaps& m, const prism_ctx* ctx, cudaStream_t s) {
+    if (bf16) return backward ? launch<__nv_bfloat16, true>(a, m, ctx, s) : launch<__nv_bfloat16, false>(a, m, ctx, s);
+    return backward ? launch<__half, true>(a, m, ctx, s) : launch<__half, false>(a, m, ctx, s);
 }
 
 }  // namespace prism

@@ -31,6 +31,6 @@ struct FusedArgs {
 
 // CTA pairs of a launch over `tiles` row tiles
 inline int fused_pairs(int tiles, int sm_count) { return tiles < sm_count / 2 ? tiles : sm_count / 2; }
-cudaError_t launch_gated_fused(bool bf16, bool backward, const FusedArgs& a, const FusedMaps& m, int sm_count, cudaStream_t s);
+cudaError_t launch_gated_fused(bool bf16, bool backward, const FusedArgs& a, const FusedMaps& m, const prism_ctx* ctx, cudaStream_t s);
 
 }  // namespace prism

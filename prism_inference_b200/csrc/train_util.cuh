@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "host_util.h"
 
@@ -49,6 +51,17 @@ template <>
 PRISM_DEV void unpack2<__nv_bfloat16>(uint32_t v, float& a, float& b) {
     a = __uint_as_float(v << 16);
     b = __uint_as_float(v & 0xffff0000u);
+}
+
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once a kernel and device (`done`: the kernel's own bit
+// per device; setting it twice from two threads does no harm)
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 inline int dtype_bytes(int dtype) { return dtype == PRISM_DTYPE_F32 ? 4 : 2; }
