@@ -220,48 +220,35 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             int stage = 0, it = 0;
             uint32_t phase = 0;
             bool ok = true;
+            const uint32_t id_k = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);        // both K-major
+            const uint32_t id_x = idesc_pair(256, KIND == BACK ? 128 : a.bn, bf16, 0, 1), id_w = idesc_pair(256, a.bn, bf16, 1, 1);
             for (int u = pair; u < a.units && ok; u += pairs, ++it) {
                 const Unit t = unit_of<KIND>(a, u);
                 const int slot = it % kSlots;
                 const uint32_t acc = tmem + slot * 256;
                 if (KIND != BACK) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_cl(&bars->acc_empty[slot], ((it / kSlots) & 1) ^ 1, abort));
+                    ok = mbar_wait_w(&bars->acc_empty[slot], ((it / kSlots) & 1) ^ 1, abort);
                     if (!ok) break;
                     tc_fence_after();
                 }
                 const int kd = (a.dim + 63) / 64;
                 for (int kb = 0; kb < t.nkb; ++kb) {
                     if (KIND == BACK && kb == kd) {  // dh is on its way; g and u need the last unit's read
-                        ok = __all_sync(0xffffffffu, mbar_wait_cl(&bars->acc_empty[0], (it & 1) ^ 1, abort));
+                        ok = mbar_wait_w(&bars->acc_empty[0], (it & 1) ^ 1, abort);
                         if (!ok) break;
                         tc_fence_after();
                     }
                     if (!mbar_wait_w(&bars->full[stage], phase, abort)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + kStageA;
-                    if (KIND == XW && t.seg >= 0) {
-                        const uint32_t id = idesc_pair(256, a.bn, bf16, 1, 1);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc, sdesc_mn(sa + k * 2048, 8192), sdesc_mn(sb + k * 2048, 8192), id, (kb | k) != 0);
-                    } else if (KIND == XW) {
-                        const uint32_t id = idesc_pair(256, a.bn, bf16, 0, 1);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc, sdesc(sa + k * 32, SW128), sdesc_mn(sb + k * 2048, 8192), id, (kb | k) != 0);
-                    } else if (KIND == BACK && kb < kd) {
-                        const uint32_t id = idesc_pair(256, 128, bf16, 0, 1);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc + 256 + (it & 1) * 128, sdesc(sa + k * 32, SW128), sdesc_mn(sb + k * 2048, 8192),
-                                          id, (kb | k) != 0);
-                    } else {
-                        const uint32_t id = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_pair_ss_w(acc, sdesc(sa + k * 32, SW128), sdesc(sb + k * 32, SW128), id,
-                                          (KIND == BACK ? (kb - kd) | k : kb | k) != 0);
-                    }
+                    if (KIND == XW && t.seg >= 0)
+                        mma_pair_x4<128, 128>(acc, desc_lo(sa, 8192), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_w, kb);
+                    else if (KIND == XW)
+                        mma_pair_x4<2, 128>(acc, desc_lo(sa), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_x, kb);
+                    else if (KIND == BACK && kb < kd)
+                        mma_pair_x4<2, 128>(acc + 256 + (it & 1) * 128, desc_lo(sa), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_x, kb);
+                    else
+                        mma_pair_x4<2, 2>(acc, desc_lo(sa), kDescHi128, desc_lo(sb), kDescHi128, id_k, KIND == BACK ? kb - kd : kb);
                     mma_commit_pair_w(&bars->empty[stage]);
                     if (++stage == kStages) {
                         stage = 0;
@@ -367,7 +354,7 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                     if (g) {  // everything read: the next unit's products may come
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_peer(acc_empty0);
+                        if (lane == 0) mbar_arrive_pair(acc_empty0);
                     }
                     if (a.act == kActSilu) grad_cols<T, kActSilu>(rg, ru, rd, bias + g, bias + 32 + g, dg, du, h + g / 2);
                     else if (a.act == kActGelu) grad_cols<T, kActGelu>(rg, ru, rd, bias + g, bias + 32 + g, dg, du, h + g / 2);
@@ -476,7 +463,7 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_peer(slot ? acc_empty1 : acc_empty0);
+            if (lane == 0) mbar_arrive_pair(slot ? acc_empty1 : acc_empty0);
         }
         if (lane == 0) tma_store_wait0();
     }
@@ -488,32 +475,43 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
 }
 
 // ---- joining the partial sums ------------------------------------------------------------------
-// dW from the splits' sums [split][3][hidden][dim] by 32 x 32 tiles, the third weight transposed; behind
-// those CTAs, db from the warps' column sums [n_sums][2 hidden] and [n_dy][dim], 32 columns a CTA.
+// dW from the splits' sums [split][3][hidden][dim] by 32 x 32 tiles, four columns a thread, the third
+// weight transposed; behind those CTAs, db from the warps' column sums [n_sums][2 hidden] and
+// [n_dy][dim], 32 columns a CTA: 32 threads deep, each over every 32nd row, then the 32 in order.  Bound
+// by latency: single loads 8 deep took 45 us for 592 rows of sums, this 12.
+PRISM_DEV float4 operator+(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+template <typename T>
+PRISM_DEV void store4(T* out, const float4& v) { *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)); }
+
 template <typename T>
 __global__ void __launch_bounds__(256)
     fold_kernel(const float* dw, int splits, const float* sums, int n_sums, const float* sums_dy, int n_dy, int hidden, int dim,
-                T* dwg, T* dwu, T* dwd, T* dbg, T* dbu, T* dbd) {
+                T* dwg, T* dwu, T* dwd, T* dbg, T* dbu, T* dbd, int aligned) {
     __shared__ float tile[32][33];
+    __shared__ float4 red[32][8];
     grid_dep_wait();
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;  // columns 4 tx .., row ty
     const int dt = (dim + 31) / 32, ht = (hidden + 31) / 32;
     int b = blockIdx.x;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (b >= 3 * dt * ht) {
-        const int cols = 2 * hidden + dim, c = (b - 3 * dt * ht) * 32 + tx;
-        float s = 0.0f;
-        if (c < 2 * hidden)
-            for (int p = ty; p < n_sums; p += 8) s += sums[(int64_t)p * 2 * hidden + c];
-        else if (c < cols)
-            for (int p = ty; p < n_dy; p += 8) s += sums_dy[(int64_t)p * dim + c - 2 * hidden];
-        tile[ty][tx] = s;
+        // dim and hidden are multiples of 8: four columns are of one vector
+        const int cols = 2 * hidden + dim, c = (b - 3 * dt * ht) * 32 + 4 * tx;
+        const float* src = c < 2 * hidden ? sums + c : sums_dy + c - 2 * hidden;
+        const int n = c < 2 * hidden ? n_sums : c < cols ? n_dy : 0, pitch = c < 2 * hidden ? 2 * hidden : dim;
+#pragma unroll 4
+        for (int p = ty; p < n; p += 32) s = s + *reinterpret_cast<const float4*>(src + (int64_t)p * pitch);
+        red[ty][tx] = s;
         __syncthreads();
         if (ty == 0 && c < cols) {
-            s = 0.0f;
+            s = red[0][tx];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += tile[i][tx];
+            for (int i = 1; i < 32; ++i) s = s + red[i][tx];
             T* out = c < hidden ? dbg : c < 2 * hidden ? dbu : dbd;
-            if (out) out[c < hidden ? c : c < 2 * hidden ? c - hidden : c - 2 * hidden] = from_f32<T>(s);
+            if (out) {
+                out += c < hidden ? c : c < 2 * hidden ? c - hidden : c - 2 * hidden;
+                out[0] = from_f32<T>(s.x), out[1] = from_f32<T>(s.y), out[2] = from_f32<T>(s.z), out[3] = from_f32<T>(s.w);
+            }
         }
         return;
     }
@@ -522,22 +520,25 @@ __global__ void __launch_bounds__(256)
     const int h0 = b % ht * 32, seg = b / ht;
     T* out = seg == 0 ? dwg : seg == 1 ? dwu : dwd;
     if (!out) return;
-#pragma unroll
-    for (int i = ty; i < 32; i += 8) {
-        const int h = h0 + i, d = d0 + tx;
-        float s = 0.0f;
-        if (h < hidden && d < dim) {
-            const float* p = dw + ((int64_t)seg * hidden + h) * dim + d;
-            for (int k = 0; k < splits; ++k) s += p[(int64_t)k * 3 * hidden * dim];
-            if (seg < 2) out[(int64_t)h * dim + d] = from_f32<T>(s);
+    const int h = h0 + ty, d = d0 + 4 * tx;
+    if (h < hidden && d < dim) {
+        const float* p = dw + ((int64_t)seg * hidden + h) * dim + d;
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) s = s + *reinterpret_cast<const float4*>(p + (int64_t)k * 3 * hidden * dim);
+        if (seg < 2) {
+            T* o = out + (int64_t)h * dim + d;
+            if (aligned) store4<T>(o, s);
+            else o[0] = from_f32<T>(s.x), o[1] = from_f32<T>(s.y), o[2] = from_f32<T>(s.z), o[3] = from_f32<T>(s.w);
         }
-        tile[i][tx] = s;
     }
     if (seg < 2) return;
+    tile[ty][4 * tx] = s.x, tile[ty][4 * tx + 1] = s.y, tile[ty][4 * tx + 2] = s.z, tile[ty][4 * tx + 3] = s.w;
     __syncthreads();
-    for (int i = ty; i < 32; i += 8) {
-        const int d = d0 + i, h = h0 + tx;
-        if (h < hidden && d < dim) out[(int64_t)d * hidden + h] = from_f32<T>(tile[tx][i]);
+    if (d0 + ty < dim && h0 + 4 * tx < hidden) {
+        T* o = out + (int64_t)(d0 + ty) * hidden + h0 + 4 * tx;
+        s = make_float4(tile[4 * tx][ty], tile[4 * tx + 1][ty], tile[4 * tx + 2][ty], tile[4 * tx + 3][ty]);
+        if (aligned) store4<T>(o, s);
+        else o[0] = from_f32<T>(s.x), o[1] = from_f32<T>(s.y), o[2] = from_f32<T>(s.z), o[3] = from_f32<T>(s.w);
     }
 }
 
@@ -825,11 +826,12 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             (rc = launch<T, XW>(ctx, a, m, s, who)))
             return rc;
     }
+    const int aligned = (((uintptr_t)d->dw_gate | (uintptr_t)d->dw_up | (uintptr_t)d->dw_down) & 7) == 0;
     const int blocks = 3 * ((p->dim + 31) / 32) * ((p->hidden + 31) / 32) + (2 * p->hidden + p->dim + 31) / 32;
     return cuda_rc(launch_pdl(fold_kernel<T>, dim3(blocks), dim3(256), 0, s, (const float*)dw, splits, (const float*)sums,
                               b.pairs * 8, (const float*)sums_dy, b.pairs_xw * 8, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
                               static_cast<T*>(d->dw_down), static_cast<T*>(d->db_gate), static_cast<T*>(d->db_up),
-                              static_cast<T*>(d->db_down)), who);
+                              static_cast<T*>(d->db_down), aligned), who);
 }
 
 }  // namespace

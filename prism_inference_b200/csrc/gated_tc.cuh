@@ -46,23 +46,16 @@ PRISM_DEV void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {  // one war
 PRISM_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// D (+)= A x B^T over the pair: rows 0..127 of A and of D in the leader, 128..255 in its peer; the
-// first half of B's N rows from the leader's shared memory, the second from the peer's.  Issued by one
-// elected lane of the leader's converged MMA warp.
-PRISM_DEV void mma_pair_ss_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
-        "elect.sync r|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 // Matrix descriptors as (low, high) words: the low word holds the address, so the operands of one MMA
-// after another differ by an addition there.
+// after another differ by an addition there.  K-major tiles are rows of 128 bytes (64 k; 16 k further is
+// 2 units of 16 bytes on); MN-major ones groups of 64 MN values, each [k][64] with 128 bytes a k row, 8
+// rows = 1024 bytes (the stride field), `group_bytes` from one group to the next (16 k further: 128 units).
 PRISM_DEV uint32_t desc_lo(uint32_t saddr, uint32_t group_bytes = 16) { return (saddr >> 4) | (group_bytes >> 4) << 16; }
 constexpr uint32_t kDescHi128 = (1024u >> 4) | (1u << 14) | ((uint32_t)SW128 << 29);
 constexpr uint32_t kDescHi64 = (512u >> 4) | (1u << 14) | ((uint32_t)SW64 << 29);
+// D (+)= A x B^T over the pair: rows 0..127 of A and of D in the leader, 128..255 in its peer; the
+// first half of B's N rows from the leader's shared memory, the second from the peer's.  Issued by one
+// elected lane of the leader's converged MMA warp.
 // Four MMAs (64 deep) whose descriptors advance by ASTEP, BSTEP 16-byte units, the first one adding to D
 // if `accumulate`.  One block, one elect: issued one by one, with their descriptors worked out each
 // time, 16 MMAs of N = 128 took 2000 cycles to issue for 1072 cycles of work.
@@ -113,14 +106,6 @@ PRISM_DEV uint32_t idesc_pair(int M, int N, int bf16, int a_mn, int b_mn) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// MN-major operand in 128-byte swizzle: groups of 64 MN values, each [k][64] with 128 bytes a k row (8
-// rows = 1024 bytes, the stride field), `group_bytes` from one group of 64 to the next (the leading
-// field).  16 k further is 2048 bytes on.
-PRISM_DEV uint64_t sdesc_mn(uint32_t saddr, uint32_t group_bytes) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(group_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)SW128 << 61);
-}
-
 // ---- the gate ----------------------------------------------------------------------------------
 // 1 / (1 + 2^-t): both hardware approximations are good to about 2^-22, far under the 16-bit rounding
 // that follows (tanh.approx's 2^-11 would double the error of an fp16 result).
