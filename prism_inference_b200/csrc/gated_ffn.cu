@@ -35,7 +35,8 @@ struct Cfg {
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr int kStages = KIND == BACK ? 4 : 5;
     static constexpr int kBias = KIND == BACK ? 256 : 512;  // bytes a warp
-    static constexpr int kSmem = kStages * kStage + kEpiWarps * (kOut + kBias) + 512 + 1024;
+    static constexpr int kOnes = KIND == XW ? 2048 : 0;
+    static constexpr int kSmem = kStages * kStage + kOnes + kEpiWarps * (kOut + kBias) + 512 + 1024;
 };
 constexpr int kMaxStages = 5;
 
@@ -57,7 +58,8 @@ struct Args {
     int w_tiles, k_per, k_all;  // XW: 256-row tiles of one weight's hidden axis; row blocks a split, in all
     int act;
     int first;                  // the first chunk: sums over rows start here
-    float *sums, *sums_dy;      // column sums of dg and du (BACK) and of dy (XW): [CTAs][4][2 hidden], [CTAs][4][dim]
+    float *sums, *sums_dy;      // column sums of dg and du (BACK) and of dy (XW): [CTAs][4][2 hidden], [splits][16][dim]
+    float* sums_w;              // XW: [splits][2 hidden] column sums of dg and du, or NULL
     const void* dy;             // XW: rows for the sums
     int64_t dy_stride;
     const void *b_gate, *b_up, *b_down;
@@ -125,7 +127,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
     constexpr int kStages = Cfg<KIND>::kStages, kEpiWarps = Cfg<KIND>::kEpiWarps;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_align1k(smem_raw);
-    unsigned char* s_out = smem + kStages * kStage;
+    unsigned char* s_ones = smem + kStages * kStage;
+    unsigned char* s_out = s_ones + Cfg<KIND>::kOnes;
     unsigned char* s_bias = s_out + kEpiWarps * kOut;
     Bars* bars = reinterpret_cast<Bars*>(s_bias + kEpiWarps * Cfg<KIND>::kBias);
     volatile int* abort = &bars->abort;
@@ -133,9 +136,15 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
     const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // Accumulators: two of 256 columns.  BACK has [g | u] in columns 0 .. 255 and dh in one of two slots
     // of 128 behind them, so that a unit's dh is computed while the epilogue still reads the unit before.
-    constexpr int kSlots = KIND == BACK ? 1 : 2;
+    // XW that also sums dg's and du's columns (sums_w) has the sums behind one accumulator.
+    const int slots = KIND == BACK || (KIND == XW && a.sums_w) ? 1 : 2;
     constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
 
+    if (KIND == XW) {
+        const uint32_t one = bf16 ? 0x3f803f80u : 0x3c003c00u;
+        for (int i = threadIdx.x; i < Cfg<KIND>::kOnes / 4; i += Cfg<KIND>::kThreads) reinterpret_cast<uint32_t*>(s_ones)[i] = one;
+        fence_async_shared();
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&bars->full[s], 1);
@@ -222,12 +231,13 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             bool ok = true;
             const uint32_t id_k = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);        // both K-major
             const uint32_t id_x = idesc_pair(256, KIND == BACK ? 128 : a.bn, bf16, 0, 1), id_w = idesc_pair(256, a.bn, bf16, 1, 1);
+            const uint32_t id_1 = idesc_pair(256, 32, bf16, 1, 0);
             for (int u = pair; u < a.units && ok; u += pairs, ++it) {
                 const Unit t = unit_of<KIND>(a, u);
-                const int slot = it % kSlots;
+                const int slot = it % slots;
                 const uint32_t acc = tmem + slot * 256;
                 if (KIND != BACK) {
-                    ok = mbar_wait_w(&bars->acc_empty[slot], ((it / kSlots) & 1) ^ 1, abort);
+                    ok = mbar_wait_w(&bars->acc_empty[slot], ((it / slots) & 1) ^ 1, abort);
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -241,8 +251,11 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                     if (!mbar_wait_w(&bars->full[stage], phase, abort)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + kStageA;
-                    if (KIND == XW && t.seg >= 0)
+                    if (KIND == XW && t.seg >= 0) {
                         mma_pair_x4<128, 128>(acc, desc_lo(sa, 8192), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_w, kb);
+                        if (a.sums_w && t.seg < 2 && t.nt == 0)  // times ones: the bias gradient, on tensor time to spare
+                            mma_pair_x4<128, 2>(tmem + 256, desc_lo(sa, 8192), kDescHi128, desc_lo(smem_u32(s_ones)), kDescHi128, id_1, kb);
+                    }
                     else if (KIND == XW)
                         mma_pair_x4<2, 128>(acc, desc_lo(sa), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_x, kb);
                     else if (KIND == BACK && kb < kd)
@@ -269,9 +282,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         const uint32_t acc_empty0 = peer_addr(smem_u32(&bars->acc_empty[0]), 0);
         const uint32_t acc_empty1 = peer_addr(smem_u32(&bars->acc_empty[1]), 0);
-        // Column sums of this warp's rows: BACK of dg and du, XW of dy.  Each warp has columns of its own.
-        float* sums = KIND == BACK ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden)
-                      : KIND == XW ? a.sums_dy + ((int64_t)blockIdx.x * 4 + quad) * a.dim : nullptr;
+        // BACK: column sums of this warp's rows of dg and du.  Each warp has columns of its own.
+        float* sums = KIND == BACK ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden) : nullptr;
         float next_g = 0.0f, next_u = 0.0f;  // BACK: the next unit's biases of column `lane`
         if (KIND == BACK) {
             if (a.first) {
@@ -282,15 +294,11 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             next_g = ld_bias<T>(a.b_gate, c, a.hidden);
             next_u = ld_bias<T>(a.b_up, c, a.hidden);
         }
-        if (KIND == XW && a.first && a.sums_dy) {
-            for (int c = lane; c < a.dim; c += 32)
-                if (((c >> 5) & 1) == half) sums[c] = 0.0f;
-        }
         __syncwarp();
         int it = 0;
         for (int u = pair; u < a.units; u += pairs, ++it) {
             const Unit t = unit_of<KIND>(a, u);
-            const int slot = it % kSlots;
+            const int slot = it % slots;
             const int row = t.mt * 256 + rank * 128 + quad * 32;
             const int cols = KIND == BACK ? 32 : KIND == UP ? 64 : a.bn / 2;  // this warp's
             const int col0 = (KIND == BACK || KIND == UP ? t.nt * 128 : t.nt * a.bn) + half * cols;
@@ -312,30 +320,46 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             } else if (KIND == DOWN) {
                 for (int i = lane; i < cols; i += 32) bias[i] = ld_bias<T>(a.b_down, col0 + i, a.dim);
             }
-            if (KIND == XW && t.seg < 0 && t.nt == 0 && a.sums_dy) {  // while the unit's products run
-                const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
-                for (int c = half * 32; c < a.dim; c += 64) {
-                    const int cc = c + 2 * (lane & 15);
-                    uint32_t v[16];
+            if (KIND == XW && a.sums_dy && t.seg == 2 && t.mt == 0) {
+                // dy's column sums over the split's rows while the products over the same rows run (and bring them to
+                // L2): every 16th row a warp, 8 columns a lane
+                const int c = t.nt * a.bn + 8 * lane, r1 = min(a.rows, (t.k0 + t.nkb) * 64);
+                if (8 * lane < a.bn && c < a.dim) {
+                    const T* dy = static_cast<const T*>(a.dy) + c;
+                    float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    const int w = rank * kEpiWarps + warp - 2;
+                    for (int r = t.k0 * 64 + w; r < r1; r += 16 * 8) {
+                        uint4 v[8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        v[i] = row + (lane >> 4) + 2 * i < a.rows && cc < a.dim
-                                   ? *reinterpret_cast<const uint32_t*>(dy + (int64_t)(2 * i) * a.dy_stride + cc) : 0u;
-                    float s0 = 0.0f, s1 = 0.0f;
+                        for (int i = 0; i < 8; ++i)
+                            v[i] = r + 16 * i < r1 ? *reinterpret_cast<const uint4*>(dy + (int64_t)(r + 16 * i) * a.dy_stride)
+                                                   : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float f0, f1;
-                        unpack2<T>(v[i], f0, f1);
-                        s0 += f0;
-                        s1 += f1;
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t q[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                float f0, f1;
+                                unpack2<T>(q[j], f0, f1);
+                                s[2 * j] += f0;
+                                s[2 * j + 1] += f1;
+                            }
+                        }
                     }
-                    s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
-                    s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
-                    if (cc < a.dim) atomicAdd(sums + cc + (lane >> 4), lane < 16 ? s0 : s1);
+                    float4* out = reinterpret_cast<float4*>(a.sums_dy + ((int64_t)t.split * 16 + w) * a.dim + c);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float4 o = make_float4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
+                        if (!a.first) {
+                            const float4 p = out[j];
+                            o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+                        }
+                        out[j] = o;
+                    }
                 }
             }
             __syncwarp();
-            const bool got = mbar_wait_w(&bars->acc_full[slot], (it / kSlots) & 1, abort);
+            const bool got = mbar_wait_w(&bars->acc_full[slot], (it / slots) & 1, abort);
             if (!got) break;
             tc_fence_after();
             const uint32_t acc = tmem + lane_addr + slot * 256;
@@ -387,6 +411,15 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                     tma_store_commit();
                 }
                 continue;
+            }
+            if (KIND == XW && a.sums_w && t.seg >= 0 && t.seg < 2 && t.nt == 0 && half == 0) {
+                uint32_t r[16];  // 32 equal columns
+                tmem_ld16(tmem + lane_addr + 256, r);
+                tmem_ld_wait();
+                if (row + lane < a.hidden) {
+                    float* p = a.sums_w + ((int64_t)t.split * 2 + t.seg) * a.hidden + row + lane;
+                    *p = a.first ? __uint_as_float(r[0]) : *p + __uint_as_float(r[0]);
+                }
             }
             for (int g = 0; g < cols; g += 32) {
                 const int c = col0 + g;
@@ -609,7 +642,9 @@ inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 struct BackPlan {
     bool fused;
     int64_t chunk;
-    int splits, pairs, pairs_xw;  // CTA pairs of the first chunk's launches: 8 rows of column sums each
+    int splits, pairs;            // pairs: of BACK's first launch
+    int n_sums, n_dy;             // rows of the column sums of dg and du (a split's or a warp's) and of dy (a CTA's or a
+                                  // split's warp's)
     size_t p_bytes, dw_bytes, sum_bytes;
     size_t total() const { return p_bytes + dw_bytes + sum_bytes; }
 };
@@ -622,11 +657,11 @@ BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     b.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kb, (ctx->sm_count / 2) / tiles));
     b.fused = p->dim <= kFusedMaxDim;
     b.pairs = (int)std::min<int64_t>(ctx->sm_count / 2, (b.chunk + 255) / 256 * (b.fused ? 1 : (p->hidden + 127) / 128));
-    const int64_t x_units = (b.chunk + 255) / 256 * ((p->dim + bn - 1) / bn), k_per = (kb + b.splits - 1) / b.splits;
-    b.pairs_xw = b.fused ? b.pairs : (int)std::min<int64_t>(ctx->sm_count / 2, x_units + tiles * ((kb + k_per - 1) / k_per));
     b.p_bytes = (size_t)up_to(3 * b.chunk * p->hidden * 2, 1024);
     b.dw_bytes = (size_t)up_to((int64_t)b.splits * 3 * p->hidden * p->dim * 4, 1024);
-    b.sum_bytes = (size_t)8 * (b.pairs * 2 * (size_t)p->hidden + b.pairs_xw * (size_t)p->dim) * 4;
+    b.n_sums = b.fused ? b.splits : 8 * b.pairs;
+    b.n_dy = b.fused ? 2 * b.pairs : 16 * b.splits;
+    b.sum_bytes = (b.n_sums * 2 * (size_t)p->hidden + b.n_dy * (size_t)p->dim) * 4;
     return b;
 }
 
@@ -753,7 +788,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
     T* pbuf = static_cast<T*>(ws);
     float* dw = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes);
     float* sums = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes + b.dw_bytes);
-    float* sums_dy = sums + (size_t)b.pairs * 8 * 2 * p->hidden;
+    float* sums_dy = sums + (size_t)b.n_sums * 2 * p->hidden;
     int rc, splits = 1;
     for (int64_t r0 = 0; r0 < p->rows; r0 += b.chunk) {
         const int rows = (int)std::min(b.chunk, p->rows - r0);
@@ -783,19 +818,17 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             FusedMaps fm;
             fused_args(ctx, p, w, rows, f);
             f.first = r0 == 0;
-            f.sums = sums;
             f.sums_dy = sums_dy;
-            f.dy = dyc;
-            f.dy_stride = dys;
             if ((rc = fused_maps(p, w, xc, xs, rows, 64, fm)) ||
                 (rc = make_map(&fm.dy, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
                 (rc = make_map(&fm.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 32, 128, kSw64)) ||
-                (rc = make_map(&fm.wg_mn, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
-                (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
+                (rc = make_map(&fm.wg_mn, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 32, kSw128)) ||
+                (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 32, kSw128)) ||
                 (rc = make_map(&fm.p, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 32, kSw128)) ||
                 (rc = make_map(&fm.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
                 (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx, s), who)))
                 return rc;
+            a.sums_w = sums;
             a.sums_dy = nullptr;
         } else {
             if ((rc = make_map(&m.a0, xc, p->dtype, p->dim, rows, 0, xs, 64, 128, kSw128)) ||
@@ -829,7 +862,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
     const int aligned = (((uintptr_t)d->dw_gate | (uintptr_t)d->dw_up | (uintptr_t)d->dw_down) & 7) == 0;
     const int blocks = 3 * ((p->dim + 31) / 32) * ((p->hidden + 31) / 32) + (2 * p->hidden + p->dim + 31) / 32;
     return cuda_rc(launch_pdl(fold_kernel<T>, dim3(blocks), dim3(256), 0, s, (const float*)dw, splits, (const float*)sums,
-                              b.pairs * 8, (const float*)sums_dy, b.pairs_xw * 8, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
+                              b.fused ? splits : b.n_sums, (const float*)sums_dy, b.fused ? b.n_dy : 16 * splits, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
                               static_cast<T*>(d->dw_down), static_cast<T*>(d->db_gate), static_cast<T*>(d->db_up),
                               static_cast<T*>(d->db_down), aligned), who);
 }

@@ -5,10 +5,9 @@
 // hidden values never leave the SM forward.  Per step:
 //   forward   [g | u] = x [Wg | Wu]^T -> TMEM;  epilogue: h = act(g + bg) (u + bu) -> smem;  y += h Wd^T
 //   backward  [g | u] and dh = dy Wd -> TMEM;  epilogue: dg, du, h -> smem, from where TMA also stores
-//             them for the weight gradients' products, and column sums for the bias gradients;
-//             dx += dg Wg + du Wu
-// The MMA warp issues the products of step c + 1 before those that need the epilogue of step c, so the
-// tensor pipe works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3072
+//             them for the weight gradients' products;  dx += dg Wg + du Wu
+// The products of step c + 1 are issued before those that need the epilogue of step c, so the tensor pipe
+// works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3072
 // cycles of products), 80 KB backward (2850), some 30 bytes a clock; the streaming kernels of
 // gated_ffn.cu load every operand for every product and are held at the 37 to 40 that L2 gives an SM.
 #include <type_traits>
@@ -28,9 +27,11 @@ struct Cfg {
     static constexpr int kThreads = 32 * (2 + kEpiWarps + (BWD ? 1 : 4));
     static constexpr int kStep = BWD ? 64 : 128;  // hidden columns a step
     static constexpr int kCols = kStep / 4;       // of an epilogue warp
-    static constexpr int kRing = 3, kStage = BWD ? 16384 : 32768;
+    // The ring's depth hides a load's 1500 cycles; small stages keep more of it in flight.
+    static constexpr int kRing = BWD ? 6 : 3, kStage = BWD ? 8192 : 32768;
+    static constexpr int kPer = BWD ? 1 : 2;  // K-blocks of [g | u] a stage
     static constexpr int kXBytes = (BWD ? 8 : 4) * kTile;  // x, dy: four K-blocks each
-    static constexpr int kPBytes = (BWD ? 3 : 2) * kTile;  // dg, du, h, or h
+    static constexpr int kPBytes = (BWD ? 3 : 2) * kTile;  // dg, du, h of 64 columns, or h of 128
     static constexpr int kOut = BWD ? 0 : 4 * 3 * 2048;  // forward: three 32 x 32 boxes an output warp (backward: in p)
     static constexpr int kDown = BWD ? 0 : 1024;         // the output's bias
     static constexpr int kBias = 2 * kCols * 4;          // bytes an epilogue warp
@@ -40,8 +41,9 @@ struct Cfg {
     static constexpr int kAcc = 256;  // first TMEM column of [g | u (| dh)], behind the output accumulator
 };
 struct Bars {
-    uint64_t full[3], empty[3], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
+    uint64_t full[6], empty[6], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
     uint64_t p_quad[4], p_read;  // backward: a quad's rows of p are written; p's stores have read it
+    uint64_t dy_read;            // backward: dy's columns are summed
     uint64_t res_full[4][3];     // forward: a box of the residual has landed
     uint32_t tmem_base;
     int abort;
@@ -112,6 +114,7 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         for (int q = 0; q < 12; ++q) mbar_init(&bars->res_full[0][q], 1);
         for (int q = 0; q < 4; ++q) mbar_init(&bars->p_quad[q], 4);
         mbar_init(&bars->p_read, 1);
+        mbar_init(&bars->dy_read, 1);
         bars->abort = (smem_u32(smem) & 1023u) != 0;
         fence_barrier_init();
         fence_async_shared();
@@ -146,6 +149,7 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++it) {
             const int row = tile * 256 + rank * 128;
             ok = mbar_wait_w(&bars->x_empty, (it & 1) ^ 1, abort);
+            if (BWD && ok) ok = mbar_wait_w(&bars->dy_read, (it & 1) ^ 1, abort);
             if (!ok) break;
             if (lane == 0) {
                 const uint32_t bx = peer_addr(smem_u32(&bars->x_full), 0), by = peer_addr(smem_u32(&bars->y_full), 0);
@@ -161,32 +165,35 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
             uint32_t dst, bar;
             for (int c = 0; c <= steps && ok; ++c) {
                 if (c < steps) {
-                    // [g | u]: the leader brings Wg's rows, its peer Wu's; two K-blocks a stage
-                    for (int k = 0; k < kd; k += 2) {
-                        const int n = min(2, kd - k);
+                    // [g | u]: the leader brings Wg's rows, its peer Wu's
+                    for (int k = 0; k < kd; k += C::kPer) {
+                        const int n = min(C::kPer, kd - k);
                         if (next(n * C::kStep * 128, dst, bar))
                             for (int i = 0; i < n; ++i)
                                 tma_load_2d_pair(dst + i * C::kStep * 128, rank ? &maps.wu : &maps.wg, bar, (k + i) * 64, c * C::kStep);
                     }
                     // dh: 128 rows of Wd (k) at a time, this CTA's 32 hidden columns (n)
-                    if (BWD && next((kd + 1) / 2 * 8192, dst, bar))
-                        for (int k = 0; k < kd; k += 2) tma_load_2d_pair(dst + k * 4096, &maps.wd, bar, c * 64 + rank * 32, k * 64);
+                    if (BWD)
+                        for (int k = 0; k < kd; k += 2)
+                            if (next(8192, dst, bar)) tma_load_2d_pair(dst, &maps.wd, bar, c * 64 + rank * 32, k * 64);
                 }
                 if (c > 0 && !BWD) {  // y: this CTA's rows of Wd, both K-blocks of the step
                     if (next(2 * bh * 128, dst, bar))
                         for (int i = 0; i < 2; ++i) tma_load_2d_pair(dst + i * bh * 128, &maps.wd, bar, (c - 1) * 128 + i * 64, rank * bh);
                 }
-                if (c > 0 && BWD) {  // dx: the step's 64 hidden rows (k) of Wg, then Wu; this CTA's columns of dim (n)
-                    for (int s = 0; s < 2; ++s)
-                        if (next(bh * 128, dst, bar))
+                if (c > 0 && BWD) {  // dx: 32 hidden rows (k) of Wg, then Wu; this CTA's columns of dim (n)
+                    for (int s = 0; s < 4; ++s)
+                        if (next(bh * 64, dst, bar))
                             for (int n = 0; n < bh; n += 64)
-                                tma_load_2d_pair(dst + n * 128, s ? &maps.wu_mn : &maps.wg_mn, bar, rank * bh + n, (c - 1) * 64);
+                                tma_load_2d_pair(dst + n * 64, s < 2 ? &maps.wg_mn : &maps.wu_mn, bar, rank * bh + n,
+                                                 (c - 1) * 64 + (s & 1) * 32);
                 }
             }
             __syncwarp();
         }
     } else if (warp == 1) {
-        // ---- MMA issuer: the leader's, for both CTAs
+        // ---- MMA issuer: the leader's, for both CTAs.  (The ring has one consumer: two that pass over each
+        // other's stages can be two phases of a barrier apart, which its parity cannot tell from none.)
         if (rank == 0) {
             int stage = 0;
             uint32_t phase = 0, it = 0, i = 0;  // i: steps so far
@@ -215,19 +222,22 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     if (c < steps) {
                         // the epilogue has read the step before
                         mbar_wait_step(&bars->acc_empty, ((i + c) & 1) ^ 1, abort);
-                        for (int k = 0; k < kd; k += 2) {
+                        for (int k = 0; k < kd; k += C::kPer) {
                             const uint32_t b_lo = desc_lo(take());
                             mma_pair_x4<2, 2>(acc, x_lo + k * kBlk, kDescHi128, b_lo, kDescHi128, id_gu, k);
-                            if (k + 1 < kd)
+                            if (C::kPer == 2 && k + 1 < kd)
                                 mma_pair_x4<2, 2>(acc, x_lo + (k + 1) * kBlk, kDescHi128, b_lo + C::kStep * 8, kDescHi128, id_gu, 1);
                             give();
                         }
                         if (BWD) {
                             if (c == 0) mbar_wait_step(&bars->y_full, it & 1, abort);
-                            const uint32_t b_lo = desc_lo(take());
-                            for (int k = 0; k < kd; ++k)
-                                mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo + k * 256, kDescHi64, id_dh, k);
-                            give();
+                            for (int k = 0; k < kd; k += 2) {
+                                const uint32_t b_lo = desc_lo(take());
+                                mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo, kDescHi64, id_dh, k);
+                                if (k + 1 < kd)
+                                    mma_pair_x4<2, 64>(acc + 128, x_lo + (5 + k) * kBlk, kDescHi128, b_lo + 256, kDescHi64, id_dh, 1);
+                                give();
+                            }
                         }
                         mma_commit_pair_w(&bars->acc_full);
                         if (c == steps - 1) mma_commit_pair_w(&bars->x_empty);
@@ -241,8 +251,9 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                             mma_pair_x4<2, 2>(tmem, p_lo + kBlk, kDescHi128, b_lo + bh * 8, kDescHi128, id_y, 1);
                             give();
                         } else {
-                            for (int s = 0; s < 2; ++s) {
-                                mma_pair_x4<2, 128>(tmem, p_lo + s * kBlk, kDescHi128, desc_lo(take(), 8192), kDescHi128, id_dx, (c - 1) | s);
+                            for (int s = 0; s < 4; ++s) {
+                                mma_pair_x2<2, 128>(tmem, p_lo + (s >> 1) * kBlk + (s & 1) * 4, kDescHi128, desc_lo(take(), 4096), kDescHi128,
+                                                    id_dx, (c - 1) | s);
                                 give();
                             }
                         }
@@ -254,12 +265,21 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
             }
         }
     } else if (BWD && warp == 2 + kEpiWarps) {
-        // ---- stores of p: 32 rows as soon as their four warps have written them
+        // ---- stores of p: 32 rows as soon as their four warps have written them; between them, dy's column sums
+        // (db_down) from its tile in shared memory: 32 rows of 64 columns a unit, 8 columns a lane, shared out
+        // over the tile's steps
+        float* sums = a.sums_dy + (int64_t)blockIdx.x * a.dim;
+        if (a.first)
+            for (int c = lane; c < a.dim; c += 32) sums[c] = 0.0f;
+        __syncwarp();
+        const int per_step = (4 * kd + steps - 1) / steps;
         uint32_t i = 0;
-        for (int tile = pair; tile < a.tiles; tile += pairs)
+        for (int tile = pair; tile < a.tiles; tile += pairs) {
+            int unit = 0;
+            float s8[8];
             for (int c = 0; c < steps; ++c, ++i) {
                 for (int q = 0; q < 4; ++q) {
-                    mbar_wait_step(&bars->p_quad[q], i & 1, abort);
+                    mbar_wait_step(&bars->p_quad[q], i & 1, abort);  // (so dy has landed: p needs its products)
                     const int row = tile * 256 + rank * 128 + q * 32;
                     if (lane == 0 && row < a.rows) {
                         const uint32_t src = smem_u32(s_p + q * 4096);
@@ -273,7 +293,37 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     mbar_arrive(&bars->p_read);
                 }
                 __syncwarp();
+                for (int n = 0; n < per_step && unit < 4 * kd; ++n, ++unit) {
+                    const unsigned char* dy = s_x + (4 + (unit >> 2)) * kTile;
+                    if ((unit & 3) == 0) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) s8[j] = 0.0f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 32; r += 4) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(dy + sw128_off((unit & 3) * 32 + r + (lane >> 3), lane & 7));
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float f0, f1;
+                            unpack2<T>(w[j], f0, f1);
+                            s8[2 * j] += f0;
+                            s8[2 * j + 1] += f1;
+                        }
+                    }
+                    if ((unit & 3) == 3) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            s8[j] += __shfl_xor_sync(0xffffffffu, s8[j], 8);
+                            s8[j] += __shfl_xor_sync(0xffffffffu, s8[j], 16);
+                            const int col = (unit >> 2) * 64 + 8 * lane + j;
+                            if (lane < 8 && col < a.dim) sums[col] += s8[j];
+                        }
+                    }
+                }
             }
+            if (lane == 0) mbar_arrive(&bars->dy_read);
+        }
         if (lane == 0) tma_store_wait0();
     } else if (!BWD && warp >= 2 + kEpiWarps) {
         // ---- output (forward): 32 rows a warp, 32 columns at a time.  The residual's boxes come by TMA two ahead
@@ -352,23 +402,16 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         float* bias = reinterpret_cast<float*>(s_bias + (warp - 2) * C::kBias);
         const uint32_t acc_empty = peer_addr(smem_u32(&bars->acc_empty), 0), o_empty = peer_addr(smem_u32(&bars->o_empty), 0);
         const uint32_t p_full = peer_addr(smem_u32(&bars->p_full), 0);
-        // this warp's rows of column sums; it alone has its columns of them
-        float* sums = BWD ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden) : nullptr;
-        float* sums_dy = BWD ? a.sums_dy + ((int64_t)blockIdx.x * 4 + quad) * a.dim : nullptr;
-        if (BWD && a.first) {
-            for (int c = lane; c < a.hidden; c += 32)
-                if (((c >> 4) & 3) == part) sums[c] = sums[a.hidden + c] = 0.0f;
-            for (int c = lane; c < a.dim; c += 32)
-                if (((c >> 6) & 3) == part) sums_dy[c] = 0.0f;
-        }
-        __syncwarp();
-        // the biases of this warp's columns of a step, gate's then up's: a value or two a lane, loaded a step ahead
-        float next_bias[kBiasVals];
+        // The biases of this warp's columns of a step, gate's then up's: a value or two a lane, loaded a step
+        // ahead and converted when it is their turn (a conversion next to the load waits for it: 1300 cycles).
+        T next_bias[kBiasVals];
         auto load_bias = [&](int step) {
 #pragma unroll
             for (int j = 0; j < kBiasVals; ++j) {
-                const int k = lane + 32 * j;
-                next_bias[j] = ld_bias<T>(k < C::kCols ? a.b_gate : a.b_up, step * C::kStep + part * C::kCols + k % C::kCols, a.hidden);
+                const int k = lane + 32 * j, c = step * C::kStep + part * C::kCols + k % C::kCols;
+                const void* b = k < C::kCols ? a.b_gate : a.b_up;
+                next_bias[j] = from_f32<T>(0.0f);
+                if (b && c < a.hidden) next_bias[j] = static_cast<const T*>(b)[c];
             }
         };
         load_bias(0);
@@ -377,33 +420,11 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         uint32_t it = 0, i = 0;
         for (int tile = pair; tile < a.tiles; tile += pairs, ++it) {
             const int row = tile * 256 + rank * 128 + quad * 32;
-            if (BWD) {  // dy's column sums, while the first products run: 64 columns a warp
-                const T* dy = static_cast<const T*>(a.dy) + (int64_t)(row + (lane >> 4)) * a.dy_stride;
-                for (int c = part * 64; c < min(a.dim, part * 64 + 64); c += 32) {
-                    const int cc = c + 2 * (lane & 15);
-                    uint32_t v[16];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        v[r] = row + (lane >> 4) + 2 * r < a.rows && cc < a.dim
-                                   ? *reinterpret_cast<const uint32_t*>(dy + (int64_t)(2 * r) * a.dy_stride + cc) : 0u;
-                    float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float f0, f1;
-                        unpack2<T>(v[r], f0, f1);
-                        s0 += f0;
-                        s1 += f1;
-                    }
-                    s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
-                    s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
-                    if (cc < a.dim) atomicAdd(sums_dy + cc + (lane >> 4), lane < 16 ? s0 : s1);
-                }
-            }
             for (int c = 0; c < steps; ++c, ++i) {
                 const int col = c * C::kStep + part * C::kCols;
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < kBiasVals; ++j) bias[lane + 32 * j] = next_bias[j];
+                for (int j = 0; j < kBiasVals; ++j) bias[lane + 32 * j] = to_f32(next_bias[j]);
                 load_bias(c + 1 < steps ? c + 1 : 0);
                 __syncwarp();
                 mbar_wait_w(&bars->acc_full, i & 1, abort);
@@ -466,13 +487,6 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                         mbar_arrive_pair(p_full);
                         mbar_arrive(&bars->p_quad[quad]);
                     }
-                    // column sums of what was written (this warp's own rows and columns); one warp adds to an
-                    // address, in the order of its steps: the same bits every time
-                    const float2 sg = tile_column_sums<T>(smem_u32(s_p), quad * 32, part * 2, lane);
-                    const float2 su = tile_column_sums<T>(smem_u32(s_p) + kTile, quad * 32, part * 2, lane);
-                    const float v = lane & 2 ? (lane & 1 ? su.y : su.x) : (lane & 1 ? sg.y : sg.x);
-                    const int cs = col + (lane & 1) * 8 + (lane >> 2);
-                    if (cs < a.hidden) atomicAdd(sums + (lane & 2 ? a.hidden : 0) + cs, v);
                 }
             }
             if (!BWD) continue;

@@ -13,19 +13,17 @@ struct FusedMaps {
     CUtensorMap x, wg, wu, out;  // out: y or dx, box {32, 32}
     CUtensorMap residual;        // forward, where there is one: box {32, 32}
     CUtensorMap wd;              // forward: [dim][hidden], box {64, bn / 2}; backward: box {32, 128}, 64-byte swizzle
-    CUtensorMap dy, wg_mn, wu_mn, p;  // backward: boxes {64, 64} of the weights; p [3][rows][hidden], box {64, 32}
+    CUtensorMap dy, wg_mn, wu_mn, p;  // backward: boxes {64, 32} of the weights; p [3][rows][hidden] (dg, du, h), box {64, 32}
 };
 struct FusedArgs {
     int rows, dim, hidden;
     int tiles;   // of 256 rows
     int bn;      // N of the products over dim: 128 or 256
     int act;
-    int first;   // backward: the first chunk of rows, column sums start here
     const void *b_gate, *b_up, *b_down;
     int residual;  // forward: there is one
-    float *sums, *sums_dy;  // backward: [CTAs][4][2 hidden] and [CTAs][4][dim]
-    const void* dy;
-    int64_t dy_stride;
+    int first;       // backward: the first chunk of rows, dy's column sums start here
+    float* sums_dy;  // backward: [CTAs][dim]
     uint32_t* err;
 };
 

@@ -77,6 +77,20 @@ PRISM_DEV void mma_pair_x4(uint32_t d_tmem, uint32_t alo, uint32_t ahi, uint32_t
         "n"(BSTEP), "n"(2 * BSTEP), "n"(3 * BSTEP)
         : "memory");
 }
+// The same, 32 deep.
+template <int ASTEP, int BSTEP>
+PRISM_DEV void mma_pair_x2(uint32_t d_tmem, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e, t;\n\t.reg .b32 r, a1, b1;\n\t.reg .b64 x0, x1, y0, y1;\n\t"
+        "add.u32 a1, %1, %7;\n\tadd.u32 b1, %3, %8;\n\t"
+        "mov.b64 x0, {%1, %2};\n\tmov.b64 x1, {a1, %2};\n\tmov.b64 y0, {%3, %4};\n\tmov.b64 y1, {b1, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.eq.u32 t, 0, 0;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x0, y0, %5, p;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x1, y1, %5, t;\n\t}" ::"r"(d_tmem),
+        "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "n"(ASTEP), "n"(BSTEP)
+        : "memory");
+}
 // A wait of a whole converged warp without the vote on its outcome: a wait that gives up raises *abort,
 // which the role looks at once a step (MMAs issued meanwhile compute on stale but valid memory).
 PRISM_DEV void mbar_wait_step(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -204,34 +218,6 @@ PRISM_DEV uint4 pack8(const uint64_t* v) {
         o[j] = pack2<T>(a, b);
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
-}
-// Column sums of a warp's 32 rows x 16 columns in a 128-byte swizzled tile (rows row0 .., 16-byte chunks
-// chunk0, chunk0 + 1): transposing loads give lane l eight rows of column l / 4 of each chunk, four lanes
-// make a column.  Returns the first chunk's column l / 4 and the second's.
-template <typename T>
-PRISM_DEV float2 tile_column_sums(uint32_t tile, int row0, int chunk0, int lane) {
-    uint64_t s[2] = {0, 0};
-#pragma unroll
-    for (int r = 0; r < 32; r += 16) {
-        uint32_t b[4];  // 8 x 8 blocks: rows r .., r + 8 .. of the first chunk, then of the second
-        ldsm_x4_trans(tile + sw128_off(row0 + r + (lane & 15), chunk0 + (lane >> 4)), b[0], b[1], b[2], b[3]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float v0, v1;
-            unpack2<T>(b[k], v0, v1);
-            s[k >> 1] = f2_add(s[k >> 1], f2_pack(v0, v1));
-        }
-    }
-    float v[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        float a, b;
-        f2_unpack(s[k], a, b);
-        v[k] = a + b;
-        v[k] += __shfl_xor_sync(0xffffffffu, v[k], 1);
-        v[k] += __shfl_xor_sync(0xffffffffu, v[k], 2);
-    }
-    return make_float2(v[0], v[1]);
 }
 // Sums of 16 columns (as 8 pairs) over the warp's 32 rows: each step halves the columns that a lane still
 // holds (16 shuffles for 16 columns).  Lanes l and l + 1 end with column l / 2 (bits of l, high first).
