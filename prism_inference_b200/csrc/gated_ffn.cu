@@ -822,8 +822,8 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             if ((rc = fused_maps(p, w, xc, xs, rows, 64, fm)) ||
                 (rc = make_map(&fm.dy, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
                 (rc = make_map(&fm.wd, w->w_down, p->dtype, p->hidden, p->dim, 0, p->hidden, 32, 128, kSw64)) ||
-                (rc = make_map(&fm.wg_mn, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 32, kSw128)) ||
-                (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 32, kSw128)) ||
+                (rc = make_map(&fm.wg_mn, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
+                (rc = make_map(&fm.wu_mn, w->w_up, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||
                 (rc = make_map(&fm.p, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 32, kSw128)) ||
                 (rc = make_map(&fm.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
                 (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx, s), who)))

@@ -27,9 +27,9 @@ struct Cfg {
     static constexpr int kThreads = 32 * (2 + kEpiWarps + (BWD ? 1 : 4));
     static constexpr int kStep = BWD ? 64 : 128;  // hidden columns a step
     static constexpr int kCols = kStep / 4;       // of an epilogue warp
-    // The ring's depth hides a load's 1500 cycles; small stages keep more of it in flight.
-    static constexpr int kRing = BWD ? 6 : 3, kStage = BWD ? 8192 : 32768;
-    static constexpr int kPer = BWD ? 1 : 2;  // K-blocks of [g | u] a stage
+    // Large stages: the commit that gives one back costs the tensor pipe some 100 cycles (backward with six of
+    // 8 KB: 4600 cycles a step).
+    static constexpr int kRing = 3, kStage = BWD ? 16384 : 32768;
     static constexpr int kXBytes = (BWD ? 8 : 4) * kTile;  // x, dy: four K-blocks each
     static constexpr int kPBytes = (BWD ? 3 : 2) * kTile;  // dg, du, h of 64 columns, or h of 128
     static constexpr int kOut = BWD ? 0 : 4 * 3 * 2048;  // forward: three 32 x 32 boxes an output warp (backward: in p)
@@ -41,7 +41,7 @@ struct Cfg {
     static constexpr int kAcc = 256;  // first TMEM column of [g | u (| dh)], behind the output accumulator
 };
 struct Bars {
-    uint64_t full[6], empty[6], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
+    uint64_t full[3], empty[3], x_full, y_full, x_empty, acc_full, acc_empty, p_full, p_empty, o_full, o_empty;
     uint64_t p_quad[4], p_read;  // backward: a quad's rows of p are written; p's stores have read it
     uint64_t dy_read;            // backward: dy's columns are summed
     uint64_t res_full[4][3];     // forward: a box of the residual has landed
@@ -166,27 +166,25 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
             for (int c = 0; c <= steps && ok; ++c) {
                 if (c < steps) {
                     // [g | u]: the leader brings Wg's rows, its peer Wu's
-                    for (int k = 0; k < kd; k += C::kPer) {
-                        const int n = min(C::kPer, kd - k);
+                    for (int k = 0; k < kd; k += 2) {
+                        const int n = min(2, kd - k);
                         if (next(n * C::kStep * 128, dst, bar))
                             for (int i = 0; i < n; ++i)
                                 tma_load_2d_pair(dst + i * C::kStep * 128, rank ? &maps.wu : &maps.wg, bar, (k + i) * 64, c * C::kStep);
                     }
                     // dh: 128 rows of Wd (k) at a time, this CTA's 32 hidden columns (n)
-                    if (BWD)
-                        for (int k = 0; k < kd; k += 2)
-                            if (next(8192, dst, bar)) tma_load_2d_pair(dst, &maps.wd, bar, c * 64 + rank * 32, k * 64);
+                    if (BWD && next((kd + 1) / 2 * 8192, dst, bar))
+                        for (int k = 0; k < kd; k += 2) tma_load_2d_pair(dst + k * 4096, &maps.wd, bar, c * 64 + rank * 32, k * 64);
                 }
                 if (c > 0 && !BWD) {  // y: this CTA's rows of Wd, both K-blocks of the step
                     if (next(2 * bh * 128, dst, bar))
                         for (int i = 0; i < 2; ++i) tma_load_2d_pair(dst + i * bh * 128, &maps.wd, bar, (c - 1) * 128 + i * 64, rank * bh);
                 }
-                if (c > 0 && BWD) {  // dx: 32 hidden rows (k) of Wg, then Wu; this CTA's columns of dim (n)
-                    for (int s = 0; s < 4; ++s)
-                        if (next(bh * 64, dst, bar))
+                if (c > 0 && BWD) {  // dx: the step's 64 hidden rows (k) of Wg, then Wu; this CTA's columns of dim (n)
+                    for (int s = 0; s < 2; ++s)
+                        if (next(bh * 128, dst, bar))
                             for (int n = 0; n < bh; n += 64)
-                                tma_load_2d_pair(dst + n * 64, s < 2 ? &maps.wg_mn : &maps.wu_mn, bar, rank * bh + n,
-                                                 (c - 1) * 64 + (s & 1) * 32);
+                                tma_load_2d_pair(dst + n * 128, s ? &maps.wu_mn : &maps.wg_mn, bar, rank * bh + n, (c - 1) * 64);
                 }
             }
             __syncwarp();
@@ -222,22 +220,19 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                     if (c < steps) {
                         // the epilogue has read the step before
                         mbar_wait_step(&bars->acc_empty, ((i + c) & 1) ^ 1, abort);
-                        for (int k = 0; k < kd; k += C::kPer) {
+                        for (int k = 0; k < kd; k += 2) {
                             const uint32_t b_lo = desc_lo(take());
                             mma_pair_x4<2, 2>(acc, x_lo + k * kBlk, kDescHi128, b_lo, kDescHi128, id_gu, k);
-                            if (C::kPer == 2 && k + 1 < kd)
+                            if (k + 1 < kd)
                                 mma_pair_x4<2, 2>(acc, x_lo + (k + 1) * kBlk, kDescHi128, b_lo + C::kStep * 8, kDescHi128, id_gu, 1);
                             give();
                         }
                         if (BWD) {
                             if (c == 0) mbar_wait_step(&bars->y_full, it & 1, abort);
-                            for (int k = 0; k < kd; k += 2) {
-                                const uint32_t b_lo = desc_lo(take());
-                                mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo, kDescHi64, id_dh, k);
-                                if (k + 1 < kd)
-                                    mma_pair_x4<2, 64>(acc + 128, x_lo + (5 + k) * kBlk, kDescHi128, b_lo + 256, kDescHi64, id_dh, 1);
-                                give();
-                            }
+                            const uint32_t b_lo = desc_lo(take());
+                            for (int k = 0; k < kd; ++k)
+                                mma_pair_x4<2, 64>(acc + 128, x_lo + (4 + k) * kBlk, kDescHi128, b_lo + k * 256, kDescHi64, id_dh, k);
+                            give();
                         }
                         mma_commit_pair_w(&bars->acc_full);
                         if (c == steps - 1) mma_commit_pair_w(&bars->x_empty);
@@ -251,9 +246,8 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                             mma_pair_x4<2, 2>(tmem, p_lo + kBlk, kDescHi128, b_lo + bh * 8, kDescHi128, id_y, 1);
                             give();
                         } else {
-                            for (int s = 0; s < 4; ++s) {
-                                mma_pair_x2<2, 128>(tmem, p_lo + (s >> 1) * kBlk + (s & 1) * 4, kDescHi128, desc_lo(take(), 4096), kDescHi128,
-                                                    id_dx, (c - 1) | s);
+                            for (int s = 0; s < 2; ++s) {
+                                mma_pair_x4<2, 128>(tmem, p_lo + s * kBlk, kDescHi128, desc_lo(take(), 8192), kDescHi128, id_dx, (c - 1) | s);
                                 give();
                             }
                         }

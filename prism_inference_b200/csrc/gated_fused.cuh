@@ -13,7 +13,7 @@ struct FusedMaps {
     CUtensorMap x, wg, wu, out;  // out: y or dx, box {32, 32}
     CUtensorMap residual;        // forward, where there is one: box {32, 32}
     CUtensorMap wd;              // forward: [dim][hidden], box {64, bn / 2}; backward: box {32, 128}, 64-byte swizzle
-    CUtensorMap dy, wg_mn, wu_mn, p;  // backward: boxes {64, 32} of the weights; p [3][rows][hidden] (dg, du, h), box {64, 32}
+    CUtensorMap dy, wg_mn, wu_mn, p;  // backward: boxes {64, 64} of the weights; p [3][rows][hidden] (dg, du, h), box {64, 32}
 };
 struct FusedArgs {
     int rows, dim, hidden;

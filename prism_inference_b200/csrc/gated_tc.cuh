@@ -77,20 +77,6 @@ PRISM_DEV void mma_pair_x4(uint32_t d_tmem, uint32_t alo, uint32_t ahi, uint32_t
         "n"(BSTEP), "n"(2 * BSTEP), "n"(3 * BSTEP)
         : "memory");
 }
-// The same, 32 deep.
-template <int ASTEP, int BSTEP>
-PRISM_DEV void mma_pair_x2(uint32_t d_tmem, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e, t;\n\t.reg .b32 r, a1, b1;\n\t.reg .b64 x0, x1, y0, y1;\n\t"
-        "add.u32 a1, %1, %7;\n\tadd.u32 b1, %3, %8;\n\t"
-        "mov.b64 x0, {%1, %2};\n\tmov.b64 x1, {a1, %2};\n\tmov.b64 y0, {%3, %4};\n\tmov.b64 y1, {b1, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\tsetp.eq.u32 t, 0, 0;\n\t"
-        "elect.sync r|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x0, y0, %5, p;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x1, y1, %5, t;\n\t}" ::"r"(d_tmem),
-        "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "n"(ASTEP), "n"(BSTEP)
-        : "memory");
-}
 // A wait of a whole converged warp without the vote on its outcome: a wait that gives up raises *abort,
 // which the role looks at once a step (MMAs issued meanwhile compute on stale but valid memory).
 PRISM_DEV void mbar_wait_step(uint64_t* bar, uint32_t parity, volatile int* abort) {
