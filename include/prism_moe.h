@@ -314,7 +314,7 @@ typedef struct prism_gated_grads {
 
 /* y = w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down + residual, row by row; residual
  * nullable.  Products accumulate in fp32; the hidden values are rounded once to dtype, as the
- * operand of the last product, and y once.  y must not overlap x; it may be residual itself. */
+ * operand of the last product (not for a few rows), and y once.  y must not overlap x; it may be residual itself. */
 int prism_gated_ffn(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
                     const void* residual, void* y, void* workspace, size_t workspace_bytes, void* stream);
 /* The gradients of sum(dy * y) without the residual path (dy itself) from x and the weights: the
@@ -324,8 +324,8 @@ int prism_gated_ffn(prism_ctx* ctx, const prism_gated_params* p, const prism_gat
 int prism_gated_ffn_backward(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
                              const void* dy, void* dx, const prism_gated_grads* grads, void* workspace,
                              size_t workspace_bytes, void* stream);
-/* The workspace of the forward (backward = 0) or backward (1) call.  Forward: none for dim <= 256, else
- * 2 hidden bytes a row up to 1 GiB (rows go through in chunks).  Backward: 6 hidden bytes a row up to
+/* The workspace of the forward (backward = 0) or backward (1) call.  Forward: 4 hidden bytes a row for a few
+ * rows (up to 8); beyond, none for dim <= 256, else 2 hidden bytes a row up to 1 GiB (rows go through in chunks).  Backward: 6 hidden bytes a row up to
  * 1 GiB, and fp32 partial sums of the gradients. */
 int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_params* p, int backward, size_t* bytes);
 

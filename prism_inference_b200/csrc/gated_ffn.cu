@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "gated_fused.cuh"
+#include "gated_small.cuh"
 
 namespace prism {
 namespace {
@@ -723,6 +724,11 @@ int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated
     const int64_t xs = row_stride(p->x_stride, p->rows, p->dim), ys = row_stride(p->y_stride, p->rows, p->dim);
     const int64_t rs = row_stride(p->residual_stride, p->rows, p->dim);
     int rc;
+    if (is_small(p->rows, p->dim, p->hidden)) {
+        SmallArgs a{(int)p->rows, p->dim, p->hidden, p->activation, x, w->w_gate, w->b_gate, w->w_up, w->b_up, w->w_down, w->b_down,
+                    residual, xs, rs, ys, static_cast<float*>(ws), y};
+        return cuda_rc(launch_gated_small(std::is_same<T, __nv_bfloat16>::value, a, s), who);
+    }
     // dim <= 256: one kernel; 522,240 x 256, hidden 1024: FWDNEW us against 1258 of the two that follow
     for (int64_t r0 = 0; p->dim <= kFusedMaxDim && r0 < p->rows; r0 += kFusedRows) {
         const int rows = (int)std::min(kFusedRows, p->rows - r0);
@@ -788,6 +794,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
     T* pbuf = static_cast<T*>(ws);
     float* dw = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes);
     float* sums = reinterpret_cast<float*>(static_cast<char*>(ws) + b.p_bytes + b.dw_bytes);
+    const bool grads = d->dw_gate || d->db_gate || d->dw_up || d->db_up || d->dw_down || d->db_down;
     float* sums_dy = sums + (size_t)b.n_sums * 2 * p->hidden;
     int rc, splits = 1;
     for (int64_t r0 = 0; r0 < p->rows; r0 += b.chunk) {
@@ -830,6 +837,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
                 return rc;
             a.sums_w = sums;
             a.sums_dy = nullptr;
+            if (!grads) continue;
         } else {
             if ((rc = make_map(&m.a0, xc, p->dtype, p->dim, rows, 0, xs, 64, 128, kSw128)) ||
                 (rc = make_map(&m.a1, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
@@ -859,6 +867,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             (rc = launch<T, XW>(ctx, a, m, s, who)))
             return rc;
     }
+    if (!grads) return PRISM_OK;
     const int aligned = (((uintptr_t)d->dw_gate | (uintptr_t)d->dw_up | (uintptr_t)d->dw_down) & 7) == 0;
     const int blocks = 3 * ((p->dim + 31) / 32) * ((p->hidden + 31) / 32) + (2 * p->hidden + p->dim + 31) / 32;
     return cuda_rc(launch_pdl(fold_kernel<T>, dim3(blocks), dim3(256), 0, s, (const float*)dw, splits, (const float*)sums,
@@ -878,6 +887,7 @@ extern "C" int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_param
     if (rc) return rc;
     *bytes = p->rows == 0 ? 0
              : backward   ? back_plan(ctx, p).total()
+             : is_small(p->rows, p->dim, p->hidden) ? (size_t)p->rows * p->hidden * 4
              : p->dim <= kFusedMaxDim ? 0 : (size_t)chunk_rows(ctx, p->rows, 2 * (int64_t)p->hidden) * p->hidden * 2;
     return PRISM_OK;
 }

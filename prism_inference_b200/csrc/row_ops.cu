@@ -467,15 +467,31 @@ __global__ void __launch_bounds__(1024)
 
 // ---- dropout ---------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3; 2011).
-PRISM_DEV uint4 philox(uint4 c, uint2 k) {
+// The key of every round, worked out once a thread: a third of the generator's instructions otherwise.
+struct PhiloxKeys {
+    uint32_t x[10], y[10];
+    PRISM_DEV explicit PhiloxKeys(uint64_t seed) {
+#pragma unroll
+        for (int r = 0; r < 10; ++r) {
+            x[r] = (uint32_t)seed + r * 0x9E3779B9u;
+            y[r] = (uint32_t)(seed >> 32) + r * 0xBB67AE85u;
+        }
+    }
+};
+PRISM_DEV uint4 philox(uint64_t block, uint64_t offset, const PhiloxKeys& k) {
+    uint4 c = make_uint4((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32));
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t p0 = (uint64_t)0xD2511F53u * c.x, p1 = (uint64_t)0xCD9E8D57u * c.z;
-        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ k.x, (uint32_t)p1, (uint32_t)(p0 >> 32) ^ c.w ^ k.y, (uint32_t)p0);
-        k.x += 0x9E3779B9u;
-        k.y += 0xBB67AE85u;
+        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ k.x[r], (uint32_t)p1, (uint32_t)(p0 >> 32) ^ c.w ^ k.y[r], (uint32_t)p0);
     }
     return c;
+}
+// element i of a block: kept iff its 16 bits are >= t / 65536.  What it holds when dropped does not matter
+// (an infinity or NaN goes too), so a choice, not a product with 0.
+PRISM_DEV float drop(uint32_t word, int i, uint32_t t16, float x, float scale, float res) {
+    const bool keep = (i & 1 ? word : word << 16) >= t16;  // t16: threshold << 16
+    return keep ? fmaf(x, scale, res) : res;
 }
 
 struct DropArgs {
@@ -497,7 +513,8 @@ struct DropArgs {
 template <typename T, bool VEC8, bool FLAT>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
     const uint64_t seed = a.rng[0], offset = a.rng[1];
-    const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
+    const PhiloxKeys keys(seed);
+    const uint32_t t16 = a.threshold << 16;
     const int64_t n = a.rows * a.dim, blocks = (n + 7) / 8, stride = (int64_t)gridDim.x * kThreads;
     const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.residual);
     T* y = static_cast<T*>(a.y);
@@ -529,7 +546,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
             for (int u = 0; u < UNR; ++u) {
                 const int64_t b = b0 + u * stride;
                 if (b >= blocks) continue;
-                const uint4 w = philox(make_uint4((uint32_t)b, (uint32_t)(b >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)), key);
+                const uint4 w = philox(b, offset, keys);
                 const uint32_t bits[4] = {w.x, w.y, w.z, w.w};
                 if (full[u]) {
 #pragma unroll
@@ -538,9 +555,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
                             const int i = q * E + e;
-                            const uint32_t h = (i & 1) ? bits[i >> 1] >> 16 : bits[i >> 1] & 0xffffu;
-                            const float v = h >= a.threshold ? to_f32(px[u][q].v[e]) * a.scale : 0.0f;
-                            o.v[e] = from_f32<T>(res ? v + to_f32(pr[u][q].v[e]) : v);
+                            o.v[e] = from_f32<T>(drop(bits[i >> 1], i, t16, to_f32(px[u][q].v[e]), a.scale, res ? to_f32(pr[u][q].v[e]) : 0.0f));
                         }
                         *reinterpret_cast<uint4*>(y + yo[u] + q * E) = o.q;
                     }
@@ -548,11 +563,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int64_t at = b * 8 + i;
-                        if (at < n) {
-                            const uint32_t h = (i & 1) ? bits[i >> 1] >> 16 : bits[i >> 1] & 0xffffu;
-                            const float v = h >= a.threshold ? to_f32(x[at]) * a.scale : 0.0f;
-                            y[at] = from_f32<T>(res ? v + to_f32(res[at]) : v);
-                        }
+                        if (at < n) y[at] = from_f32<T>(drop(bits[i >> 1], i, t16, to_f32(x[at]), a.scale, res ? to_f32(res[at]) : 0.0f));
                     }
                 }
             }
@@ -561,17 +572,14 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
             for (int u = 0; u < UNR; ++u) {
                 const int64_t b = b0 + u * stride;
                 if (b >= blocks) break;
-                const uint4 w = philox(make_uint4((uint32_t)b, (uint32_t)(b >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)), key);
+                const uint4 w = philox(b, offset, keys);
                 const uint32_t bits[4] = {w.x, w.y, w.z, w.w};
                 int64_t r = (b * 8) / a.dim;
                 int c = (int)(b * 8 - r * a.dim);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (r < a.rows) {
-                        const uint32_t h = (i & 1) ? bits[i >> 1] >> 16 : bits[i >> 1] & 0xffffu;
-                        const float v = h >= a.threshold ? to_f32(x[r * a.xs + c]) * a.scale : 0.0f;
-                        y[r * a.ys + c] = from_f32<T>(res ? v + to_f32(res[r * a.rs + c]) : v);
-                    }
+                    if (r < a.rows)
+                        y[r * a.ys + c] = from_f32<T>(drop(bits[i >> 1], i, t16, to_f32(x[r * a.xs + c]), a.scale, res ? to_f32(res[r * a.rs + c]) : 0.0f));
                     if (++c == a.dim) {
                         c = 0;
                         ++r;
@@ -636,6 +644,9 @@ int check_norm(const char* who, const prism_norm_params* p) {
     if (p->dim > kNormMaxDim) return fail(PRISM_E_UNSUPPORTED, "%s: dim %d above %d", who, p->dim, kNormMaxDim);
     return PRISM_OK;
 }
+int check_param(const char* who, const char* name, const void* t, int dtype) {
+    return t && (uintptr_t)t % dtype_bytes(dtype) ? fail(PRISM_E_ALIGN, "%s: %s is not aligned to its type", who, name) : PRISM_OK;
+}
 int check_stride(const char* who, const char* name, const void* t, int64_t stride, int64_t rows, int dim, int es) {
     if (!t) return PRISM_OK;
     if ((uintptr_t)t % es) return fail(PRISM_E_ALIGN, "%s: %s is not aligned to its type", who, name);
@@ -671,7 +682,11 @@ extern "C" int prism_layer_norm(prism_ctx* ctx, const prism_norm_params* p, cons
     if (!x || !y) return fail(PRISM_E_ARG, "prism_layer_norm: NULL argument");
     const int es = dtype_bytes(p->dtype);
     if ((rc = check_stride("prism_layer_norm", "x", x, p->x_stride, p->rows, p->dim, es)) ||
-        (rc = check_stride("prism_layer_norm", "y", y, p->y_stride, p->rows, p->dim, es)))
+        (rc = check_stride("prism_layer_norm", "y", y, p->y_stride, p->rows, p->dim, es)) ||
+        (rc = check_param("prism_layer_norm", "weight", weight, p->param_dtype)) ||
+        (rc = check_param("prism_layer_norm", "bias", bias, p->param_dtype)) ||
+        (rc = check_param("prism_layer_norm", "mean", mean, PRISM_DTYPE_F32)) ||
+        (rc = check_param("prism_layer_norm", "rstd", rstd, PRISM_DTYPE_F32)))
         return rc;
     if (bad_alias(y, p->y_stride, x, p->x_stride, p->rows, p->dim, es))
         return fail(PRISM_E_ARG, "prism_layer_norm: y overlaps x");
@@ -710,6 +725,10 @@ extern "C" int prism_layer_norm_backward(prism_ctx* ctx, const prism_norm_params
     if (!ctx || !p) return fail(PRISM_E_ARG, "%s: NULL argument", who);
     int rc = check_norm(who, p);
     if (rc) return rc;
+    if ((rc = check_param(who, "weight", weight, p->param_dtype)) || (rc = check_param(who, "dweight", dweight, p->param_dtype)) ||
+        (rc = check_param(who, "dbias", dbias, p->param_dtype)) || (rc = check_param(who, "mean", mean, PRISM_DTYPE_F32)) ||
+        (rc = check_param(who, "rstd", rstd, PRISM_DTYPE_F32)))
+        return rc;
     DeviceGuard g(ctx->device);
     if (p->rows == 0) {  // no rows: the sums are zero
         const size_t n = (size_t)p->dim * dtype_bytes(p->param_dtype);

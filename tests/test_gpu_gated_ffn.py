@@ -48,8 +48,9 @@ def backward(ctx, x, w, b, dy, dx, grads, **kw):
     return ctx.gated_ffn_backward(x, *w, dy, dx, b_gate=b[0], b_up=b[1], **grads, **kw)
 
 
-SHAPES = [(1, 8, 8), (1, 256, 1024), (3, 64, 64), (16, 256, 512), (17, 128, 136), (64, 256, 1024), (129, 128, 512), (130, 72, 200),
-          (257, 256, 256), (300, 264, 328), (1000, 128, 512), (77, 1000, 2744), (515, 520, 72), (5, 1024, 4096), (19000, 64, 128)]
+SHAPES = [(1, 8, 8), (2, 264, 40), (4, 256, 1024), (8, 1000, 2744), (9, 256, 512), (1, 256, 1024), (3, 64, 64), (16, 256, 512), (17, 128, 136), (64, 256, 1024), (129, 128, 512), (130, 72, 200),
+          (257, 256, 256), (300, 264, 328), (1000, 128, 512), (77, 1000, 2744), (515, 520, 72), (5, 1024, 4096), (19000, 64, 128),
+          (19000, 16, 9600)]  # the last one's backward pass goes through in two chunks of rows
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
@@ -85,8 +86,20 @@ def test_backward(prism_ctx, dtype, shape, kind, pad):
     assert pad_untouched(dx)
 
 
-def test_backward_gradients_are_optional(prism_ctx):
-    R, D, H = 200, 128, 256
+def test_forward_in_chunks(prism_ctx):
+    """dim > 256 and a hidden layer so wide that the rows go through in two chunks."""
+    R, D, H = 19000, 264, 14344
+    x, (w, b) = rand((R, D), F16, 1), weights(D, H, F16)
+    y = empty((R, D), F16)
+    forward(prism_ctx, x, w, b, y, residual=x)
+    for part in (slice(0, 300), slice(18800, R)):
+        want, tol = ref.gated(x[part], w, b, x[part], "gelu", F16)
+        ref.check(y[part], want, tol, "y")
+
+
+@pytest.mark.parametrize("shape", [(200, 128, 256), (200, 264, 72)])
+def test_backward_gradients_are_optional(prism_ctx, shape):
+    R, D, H = shape
     x, dy = rand((R, D), BF16, 1), rand((R, D), BF16, 2)
     w, b = weights(D, H, BF16)
     dx, grads = empty((R, D), BF16), grads_like(w, H, D)
@@ -111,8 +124,7 @@ def test_three_dimensions_and_residual_in_place(prism_ctx):
 
 def test_nonfinite_rows_stay_in_their_row(prism_ctx):
     """An infinity or a NaN in one row reaches that row's output only, also across a chunk's border."""
-    for R in (300, 19000):
-        D, H = 64, 128
+    for R, D, H in ((300, 64, 128), (19000, 16, 9600)):
         x = rand((R, D), F16, 1)
         w, b = weights(D, H, F16)
         y, y2 = torch.empty_like(x), torch.empty_like(x)
