@@ -239,7 +239,8 @@ int prism_ctx_status(prism_ctx* ctx, void* stream);
  * calls on different streams, threads or captured graphs share nothing unless the caller
  * gives them the same workspace.  The same inputs give the same bits (no atomics).
  * Calls are stream-ordered, never synchronise, never allocate and can be captured into a
- * CUDA graph.  rows == 0 is a no-op (the gradients of parameters become zero). */
+ * CUDA graph.  rows == 0 is a no-op (the gradients of parameters become zero).  A bounded device
+ * wait of the gated kernels that gives up is reported by prism_ctx_status. */
 enum prism_dtype { PRISM_DTYPE_F16 = 0, PRISM_DTYPE_BF16 = 1, PRISM_DTYPE_F32 = 2 };
 
 /* dtype: x, y, dy, add, dx.  param_dtype: weight, bias, dweight, dbias; dtype or fp32.

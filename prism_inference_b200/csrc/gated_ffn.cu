@@ -56,6 +56,7 @@ struct Args {
     int m_tiles, n_tiles;       // 256-row tiles; column tiles (128 hidden for UP / BACK, bn else)
     int bn;                     // N of an output tile over dim: 256 or 128
     int units, x_units;         // XW: the first x_units are dx tiles, the others dW tiles
+    int w_each[2];              // XW: dW tiles a pair takes, where it has one dx tile more than the others [1] or not
     int w_tiles, k_per, k_all;  // XW: 256-row tiles of one weight's hidden axis; row blocks a split, in all
     int act;
     int first;                  // the first chunk: sums over rows start here
@@ -104,6 +105,31 @@ PRISM_DEV Unit unit_of(const Args& a, int u) {
     }
     return r;
 }
+
+// The units of a pair, the same on every role: every pairs-th one.  XW's dW tiles go round the pairs w_each[1]
+// times, then round those that have a dx tile less up to w_each[0] times (the two differ in depth: 2051
+// rows of 1000 x 2744 in plain turns left the last pairs idle a third of the time, 140 against 128 us).
+// Turns, not runs, so that pairs work on neighbouring tiles at a time and share their operands in L2.
+template <int KIND>
+struct Walk {
+    int pair, pairs, n, n_x, x_units, more, w_all;
+    PRISM_DEV static int turns(int units, int first, int step) { return units > first ? (units - first + step - 1) / step : 0; }
+    PRISM_DEV Walk(const Args& a, int pair_, int pairs_) : pair(pair_), pairs(pairs_), x_units(a.x_units) {
+        n = n_x = turns(KIND == XW ? a.x_units : a.units, pair, pairs);
+        if (KIND == XW) {
+            const int n_w = a.units - a.x_units;
+            more = a.x_units % pairs;  // pairs with a dx tile more come first
+            w_all = a.w_each[1];
+            n += min(w_all, turns(n_w, pair, pairs));
+            if (pair >= more) n += min(a.w_each[0] - w_all, turns(n_w - w_all * pairs, pair - more, pairs - more));
+        }
+    }
+    PRISM_DEV int unit(int i) const {
+        if (KIND != XW || i < n_x) return pair + i * pairs;
+        i -= n_x;
+        return x_units + (i < w_all ? i * pairs + pair : w_all * pairs + (i - w_all) * (pairs - more) + pair - more);
+    }
+};
 
 // A 32 x 32 box of a warp's rows: this lane's row as 16 packed pairs into 64-byte swizzled rows.
 PRISM_DEV void stage_row64(unsigned char* buf, int lane, const uint32_t (&v)[16]) {
@@ -166,6 +192,7 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
+    const Walk<KIND> walk(a, pair, pairs);
     grid_dep_wait();
 
     if (warp == 0) {
@@ -173,8 +200,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int u = pair; u < a.units && ok; u += pairs) {
-            const Unit t = unit_of<KIND>(a, u);
+        for (int i = 0; i < walk.n && ok; ++i) {
+            const Unit t = unit_of<KIND>(a, walk.unit(i));
             const int kd = (a.dim + 63) / 64, kh = (a.hidden + 63) / 64;
             const int bh = a.bn / 2;  // this CTA's share of an N tile over dim
             for (int kb = 0; kb < t.nkb; ++kb) {
@@ -233,8 +260,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             const uint32_t id_k = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);        // both K-major
             const uint32_t id_x = idesc_pair(256, KIND == BACK ? 128 : a.bn, bf16, 0, 1), id_w = idesc_pair(256, a.bn, bf16, 1, 1);
             const uint32_t id_1 = idesc_pair(256, 32, bf16, 1, 0);
-            for (int u = pair; u < a.units && ok; u += pairs, ++it) {
-                const Unit t = unit_of<KIND>(a, u);
+            for (; it < walk.n && ok; ++it) {
+                const Unit t = unit_of<KIND>(a, walk.unit(it));
                 const int slot = it % slots;
                 const uint32_t acc = tmem + slot * 256;
                 if (KIND != BACK) {
@@ -297,8 +324,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
         }
         __syncwarp();
         int it = 0;
-        for (int u = pair; u < a.units; u += pairs, ++it) {
-            const Unit t = unit_of<KIND>(a, u);
+        for (; it < walk.n; ++it) {
+            const Unit t = unit_of<KIND>(a, walk.unit(it));
             const int slot = it % slots;
             const int row = t.mt * 256 + rank * 128 + quad * 32;
             const int cols = KIND == BACK ? 32 : KIND == UP ? 64 : a.bn / 2;  // this warp's
@@ -308,8 +335,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                 __syncwarp();
                 bias[lane] = next_g;
                 bias[32 + lane] = next_u;
-                const int c = (u + pairs) % a.n_tiles * 128 + half * 32 + lane;
-                if (u + pairs < a.units) {
+                const int c = walk.unit(it + 1) % a.n_tiles * 128 + half * 32 + lane;
+                if (it + 1 < walk.n) {
                     next_g = ld_bias<T>(a.b_gate, c, a.hidden);
                     next_u = ld_bias<T>(a.b_up, c, a.hidden);
                 }
@@ -666,6 +693,19 @@ BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     return b;
 }
 
+// XW's dW tiles over `pairs` CTA pairs: the least depth a pair that holds them all.
+void share_out(Args& a, int pairs) {
+    const int64_t kx = 2 * ((a.hidden + 63) / 64), n_w = a.units - a.x_units, more = a.x_units % pairs, all = a.x_units / pairs;
+    const auto each = [&](int64_t depth, int64_t dx) { return std::max<int64_t>(0, (depth - dx * kx) / a.k_per); };
+    int64_t lo = 0, hi = (all + 1) * kx + n_w * a.k_per;  // lo: too little, hi: enough
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        (more * each(mid, all + 1) + (pairs - more) * each(mid, all) >= n_w ? hi : lo) = mid;
+    }
+    a.w_each[1] = (int)std::min(n_w, each(hi, all + 1));
+    a.w_each[0] = (int)std::max<int64_t>(a.w_each[1], std::min(n_w, each(hi, all)));
+}
+
 int check_gated(const char* who, const prism_gated_params* p) {
     if (p->dtype != PRISM_DTYPE_F16 && p->dtype != PRISM_DTYPE_BF16)
         return fail(dtype_known(p->dtype) ? PRISM_E_UNSUPPORTED : PRISM_E_ARG, "%s: dtype %d (fp16 or bf16)", who, p->dtype);
@@ -856,6 +896,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
         const int here = (a.k_all + a.k_per - 1) / a.k_per;
         if (r0 == 0) splits = here;  // the first chunk is the largest: it writes every split's sums
         a.units = a.x_units + 3 * a.w_tiles * a.n_tiles * here;
+        share_out(a, std::min(a.units, ctx->sm_count / 2));
         if ((rc = make_map(&m.p_k, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 128, kSw128)) ||
             (rc = make_map(&m.p_mn, pbuf, p->dtype, p->hidden, rows, 3, p->hidden, 64, 64, kSw128)) ||
             (rc = make_map(&m.b0, w->w_gate, p->dtype, p->dim, p->hidden, 0, p->dim, 64, 64, kSw128)) ||

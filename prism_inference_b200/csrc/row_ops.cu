@@ -765,11 +765,8 @@ extern "C" int prism_layer_norm_backward(prism_ctx* ctx, const prism_norm_params
             constexpr int kTeam = decltype(team)::value;
             auto kernel = norm_back_kernel<decltype(quick)::value, T, kTeam, decltype(nv)::value>;
             grid = back_ctas(ctx, p->rows, kThreads / kTeam, back_ctas_per_sm<decltype(quick)::value, T, decltype(nv)::value>());
+            // at most 32 KB: a team's width grows with dim
             const size_t smem = sums && kTeam < kThreads ? (size_t)(kTeam < 32 ? kWarps : kThreads / kTeam) * p->dim * 8 : 0;
-            if (smem > 40000) {
-                int e = cuda_rc(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-                if (e) return e;
-            }
             kernel<<<grid, kThreads, smem, as_stream(stream)>>>(a);
             return cuda_rc(cudaGetLastError(), who);
         });

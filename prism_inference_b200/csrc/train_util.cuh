@@ -83,10 +83,5 @@ inline bool rows_overlap(const void* a, int64_t sa, const void* b, int64_t sb, i
     if (d < 0) d += pitch;
     return d < dim * es || pitch - d < dim * es;
 }
-// the same for flat ranges
-inline bool ranges_overlap(const void* a, size_t na, const void* b, size_t nb) {
-    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-    return a && b && na && nb && pa < pb + nb && pb < pa + na;
-}
 
 }  // namespace prism

@@ -122,6 +122,49 @@ def test_three_dimensions_and_residual_in_place(prism_ctx):
     assert torch.equal(y, r)
 
 
+@pytest.mark.parametrize("dim", [256, 264])
+def test_residual_in_place_and_column_slices_over_many_tiles(prism_ctx, dim):
+    """y as the residual itself, and x, residual and y as column slices of one buffer, with more row tiles than
+    CTA pairs: a tile's output must not reach what another still reads."""
+    R, H = 20000, 128
+    w, b = weights(dim, H, F16)
+    wide = rand((R, 3 * dim), F16, 4)
+    x, r, y = wide[:, :dim], wide[:, dim:2 * dim], wide[:, 2 * dim:]
+    want = torch.empty((R, dim), dtype=F16, device="cuda")
+    forward(prism_ctx, x.contiguous(), w, b, want, residual=r.contiguous())
+    forward(prism_ctx, x, w, b, y, residual=r)
+    assert torch.equal(y, want)
+    forward(prism_ctx, x, w, b, r, residual=r)
+    assert torch.equal(r, want)
+
+
+def test_two_graphs_at_once(prism_ctx):
+    """Two captured steps replayed on two streams at the same time share no workspace."""
+    R, D, H = 3000, 256, 512
+    w, b = weights(D, H, BF16)
+    made = []
+    for seed in (1, 2):
+        x = rand((R, D), BF16, seed)
+        y, dx, g = torch.empty_like(x), torch.empty_like(x), grads_like(w, H, D)
+        want = (torch.empty_like(x), torch.empty_like(x), grads_like(w, H, D))
+        forward(prism_ctx, x, w, b, want[0])
+        backward(prism_ctx, x, w, b, x, want[1], want[2])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            forward(prism_ctx, x, w, b, y)
+            backward(prism_ctx, x, w, b, x, dx, g)
+        made.append((graph, torch.cuda.Stream(), (y, dx, g), want, x))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, s, *_ in made:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, (y, dx, g), want, _ in made:
+        assert torch.equal(y, want[0]) and torch.equal(dx, want[1]) and all(torch.equal(g[k], want[2][k]) for k in g)
+    prism_ctx.status()
+
+
 def test_nonfinite_rows_stay_in_their_row(prism_ctx):
     """An infinity or a NaN in one row reaches that row's output only, also across a chunk's border."""
     for R, D, H in ((300, 64, 128), (19000, 16, 9600)):

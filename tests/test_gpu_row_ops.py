@@ -89,6 +89,31 @@ def test_norm_three_dimensions_and_in_place(prism_ctx):
     assert torch.equal(out[0], out[1])
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_odd_rows_in_place_and_as_column_slices(prism_ctx, dtype):
+    """Rows off 16-byte boundaries: in place, and as neighbouring column slices of one buffer, whose 16-byte
+    chunks the rows share."""
+    R, D = 3001, 101
+    x, dy = rand((R, D), dtype, 1), rand((R, D), dtype, 2)
+    w, b = rand((1, D), F32, 3)[0].contiguous(), rand((1, D), F32, 4)[0].contiguous()
+    mean, rstd = torch.empty(R, device="cuda"), torch.empty(R, device="cuda")
+    y, dx, z = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    prism_ctx.layer_norm(x, w, b, y, mean=mean, rstd=rstd)
+    prism_ctx.layer_norm_backward(x, w, mean, rstd, dy, dx, add=y)
+    prism_ctx.dropout_add(x, dy, z, 0.4, rng_of(*RNG))
+    wide = torch.full((R, 3 * D + 2), 7.0, dtype=dtype, device="cuda")
+    for src, call, want in ((x, lambda s, o: prism_ctx.layer_norm(s, w, b, o), y),
+                            (dy, lambda s, o: prism_ctx.layer_norm_backward(x, w, mean, rstd, s, o, add=y), dx),
+                            (x, lambda s, o: prism_ctx.dropout_add(s, dy, o, 0.4, rng_of(*RNG)), z)):
+        t = src.clone()
+        call(t, t)
+        assert torch.equal(t, want)
+        wide.fill_(7.0)
+        wide[:, :D] = src
+        call(wide[:, :D], wide[:, D:2 * D])
+        assert torch.equal(wide[:, D:2 * D], want) and torch.equal(wide[:, :D], src) and (wide[:, 2 * D:] == 7.0).all()
+
+
 def test_norm_constant_and_nonfinite_rows(prism_ctx):
     """A constant row has variance 0; an infinity or a NaN stays in its own row."""
     x = rand((6, 96), F32, 6)
