@@ -36,8 +36,7 @@ struct Cfg {
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr int kStages = KIND == BACK ? 4 : 5;
     static constexpr int kBias = KIND == BACK ? 256 : 512;  // bytes a warp
-    static constexpr int kOnes = KIND == XW ? 2048 : 0;
-    static constexpr int kSmem = kStages * kStage + kOnes + kEpiWarps * (kOut + kBias) + 512 + 1024;
+    static constexpr int kSmem = kStages * kStage + kEpiWarps * (kOut + kBias) + 512 + 1024;
 };
 constexpr int kMaxStages = 5;
 
@@ -61,7 +60,6 @@ struct Args {
     int act;
     int first;                  // the first chunk: sums over rows start here
     float *sums, *sums_dy;      // column sums of dg and du (BACK) and of dy (XW): [CTAs][4][2 hidden], [splits][16][dim]
-    float* sums_w;              // XW: [splits][2 hidden] column sums of dg and du, or NULL
     const void* dy;             // XW: rows for the sums
     int64_t dy_stride;
     const void *b_gate, *b_up, *b_down;
@@ -154,8 +152,7 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
     constexpr int kStages = Cfg<KIND>::kStages, kEpiWarps = Cfg<KIND>::kEpiWarps;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_align1k(smem_raw);
-    unsigned char* s_ones = smem + kStages * kStage;
-    unsigned char* s_out = s_ones + Cfg<KIND>::kOnes;
+    unsigned char* s_out = smem + kStages * kStage;
     unsigned char* s_bias = s_out + kEpiWarps * kOut;
     Bars* bars = reinterpret_cast<Bars*>(s_bias + kEpiWarps * Cfg<KIND>::kBias);
     volatile int* abort = &bars->abort;
@@ -163,15 +160,9 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
     const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // Accumulators: two of 256 columns.  BACK has [g | u] in columns 0 .. 255 and dh in one of two slots
     // of 128 behind them, so that a unit's dh is computed while the epilogue still reads the unit before.
-    // XW that also sums dg's and du's columns (sums_w) has the sums behind one accumulator.
-    const int slots = KIND == BACK || (KIND == XW && a.sums_w) ? 1 : 2;
+    constexpr int slots = KIND == BACK ? 1 : 2;
     constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
 
-    if (KIND == XW) {
-        const uint32_t one = bf16 ? 0x3f803f80u : 0x3c003c00u;
-        for (int i = threadIdx.x; i < Cfg<KIND>::kOnes / 4; i += Cfg<KIND>::kThreads) reinterpret_cast<uint32_t*>(s_ones)[i] = one;
-        fence_async_shared();
-    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&bars->full[s], 1);
@@ -259,7 +250,6 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
             bool ok = true;
             const uint32_t id_k = idesc_pair(256, KIND == DOWN ? a.bn : 256, bf16, 0, 0);        // both K-major
             const uint32_t id_x = idesc_pair(256, KIND == BACK ? 128 : a.bn, bf16, 0, 1), id_w = idesc_pair(256, a.bn, bf16, 1, 1);
-            const uint32_t id_1 = idesc_pair(256, 32, bf16, 1, 0);
             for (; it < walk.n && ok; ++it) {
                 const Unit t = unit_of<KIND>(a, walk.unit(it));
                 const int slot = it % slots;
@@ -279,11 +269,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                     if (!mbar_wait_w(&bars->full[stage], phase, abort)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + kStageA;
-                    if (KIND == XW && t.seg >= 0) {
+                    if (KIND == XW && t.seg >= 0)
                         mma_pair_x4<128, 128>(acc, desc_lo(sa, 8192), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_w, kb);
-                        if (a.sums_w && t.seg < 2 && t.nt == 0)  // times ones: the bias gradient, on tensor time to spare
-                            mma_pair_x4<128, 2>(tmem + 256, desc_lo(sa, 8192), kDescHi128, desc_lo(smem_u32(s_ones)), kDescHi128, id_1, kb);
-                    }
                     else if (KIND == XW)
                         mma_pair_x4<2, 128>(acc, desc_lo(sa), kDescHi128, desc_lo(sb, 8192), kDescHi128, id_x, kb);
                     else if (KIND == BACK && kb < kd)
@@ -439,15 +426,6 @@ __global__ void __launch_bounds__(Cfg<KIND>::kThreads, 1) __cluster_dims__(2, 1,
                     tma_store_commit();
                 }
                 continue;
-            }
-            if (KIND == XW && a.sums_w && t.seg >= 0 && t.seg < 2 && t.nt == 0 && half == 0) {
-                uint32_t r[16];  // 32 equal columns
-                tmem_ld16(tmem + lane_addr + 256, r);
-                tmem_ld_wait();
-                if (row + lane < a.hidden) {
-                    float* p = a.sums_w + ((int64_t)t.split * 2 + t.seg) * a.hidden + row + lane;
-                    *p = a.first ? __uint_as_float(r[0]) : *p + __uint_as_float(r[0]);
-                }
             }
             for (int g = 0; g < cols; g += 32) {
                 const int c = col0 + g;
@@ -671,8 +649,7 @@ struct BackPlan {
     bool fused;
     int64_t chunk;
     int splits, pairs;            // pairs: of BACK's first launch
-    int n_sums, n_dy;             // rows of the column sums of dg and du (a split's or a warp's) and of dy (a CTA's or a
-                                  // split's warp's)
+    int n_sums, n_dy;             // rows of the column sums of dg and du (a warp's) and of dy (a CTA's or a split's warp's)
     size_t p_bytes, dw_bytes, sum_bytes;
     size_t total() const { return p_bytes + dw_bytes + sum_bytes; }
 };
@@ -687,7 +664,7 @@ BackPlan back_plan(const prism_ctx* ctx, const prism_gated_params* p) {
     b.pairs = (int)std::min<int64_t>(ctx->sm_count / 2, (b.chunk + 255) / 256 * (b.fused ? 1 : (p->hidden + 127) / 128));
     b.p_bytes = (size_t)up_to(3 * b.chunk * p->hidden * 2, 1024);
     b.dw_bytes = (size_t)up_to((int64_t)b.splits * 3 * p->hidden * p->dim * 4, 1024);
-    b.n_sums = b.fused ? b.splits : 8 * b.pairs;
+    b.n_sums = 8 * b.pairs;
     b.n_dy = b.fused ? 2 * b.pairs : 16 * b.splits;
     b.sum_bytes = (b.n_sums * 2 * (size_t)p->hidden + b.n_dy * (size_t)p->dim) * 4;
     return b;
@@ -865,6 +842,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
             FusedMaps fm;
             fused_args(ctx, p, w, rows, f);
             f.first = r0 == 0;
+            f.sums = sums;
             f.sums_dy = sums_dy;
             if ((rc = fused_maps(p, w, xc, xs, rows, 64, fm)) ||
                 (rc = make_map(&fm.dy, dyc, p->dtype, p->dim, rows, 0, dys, 64, 128, kSw128)) ||
@@ -875,7 +853,6 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
                 (rc = make_map(&fm.out, dxc, p->dtype, p->dim, rows, 0, dxs, 32, 32, kSw64)) ||
                 (rc = cuda_rc(launch_gated_fused(std::is_same<T, __nv_bfloat16>::value, true, f, fm, ctx, s), who)))
                 return rc;
-            a.sums_w = sums;
             a.sums_dy = nullptr;
             if (!grads) continue;
         } else {
@@ -912,7 +889,7 @@ int backward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gate
     const int aligned = (((uintptr_t)d->dw_gate | (uintptr_t)d->dw_up | (uintptr_t)d->dw_down) & 7) == 0;
     const int blocks = 3 * ((p->dim + 31) / 32) * ((p->hidden + 31) / 32) + (2 * p->hidden + p->dim + 31) / 32;
     return cuda_rc(launch_pdl(fold_kernel<T>, dim3(blocks), dim3(256), 0, s, (const float*)dw, splits, (const float*)sums,
-                              b.fused ? splits : b.n_sums, (const float*)sums_dy, b.fused ? b.n_dy : 16 * splits, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
+                              b.n_sums, (const float*)sums_dy, b.fused ? b.n_dy : 16 * splits, p->hidden, p->dim, static_cast<T*>(d->dw_gate), static_cast<T*>(d->dw_up),
                               static_cast<T*>(d->dw_down), static_cast<T*>(d->db_gate), static_cast<T*>(d->db_up),
                               static_cast<T*>(d->db_down), aligned), who);
 }

@@ -396,6 +396,12 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
         float* bias = reinterpret_cast<float*>(s_bias + (warp - 2) * C::kBias);
         const uint32_t acc_empty = peer_addr(smem_u32(&bars->acc_empty), 0), o_empty = peer_addr(smem_u32(&bars->o_empty), 0);
         const uint32_t p_full = peer_addr(smem_u32(&bars->p_full), 0);
+        // backward: this warp's rows of the column sums of dg and du; it alone has its columns of them
+        float* sums = BWD ? a.sums + ((int64_t)blockIdx.x * 4 + quad) * (2 * a.hidden) : nullptr;
+        if (BWD && a.first)
+            for (int c = lane; c < a.hidden; c += 32)
+                if (((c >> 4) & 3) == part) sums[c] = sums[a.hidden + c] = 0.0f;
+        __syncwarp();
         // The biases of this warp's columns of a step, gate's then up's: a value or two a lane, loaded a step
         // ahead and converted when it is their turn (a conversion next to the load waits for it: 1300 cycles).
         T next_bias[kBiasVals];
@@ -481,6 +487,11 @@ __global__ void __launch_bounds__(Cfg<BWD>::kThreads, 1) __cluster_dims__(2, 1, 
                         mbar_arrive_pair(p_full);
                         mbar_arrive(&bars->p_quad[quad]);
                     }
+                    // bias gradients from the values before their rounding; one lane adds to an address, in the order of
+                    // its steps: the same bits every time
+                    const float sg = column_sum(dg, lane), su = column_sum(du, lane);
+                    const int cs = col + (lane >> 1);
+                    if (cs < a.hidden) atomicAdd(sums + (lane & 1 ? a.hidden : 0) + cs, lane & 1 ? su : sg);
                 }
             }
             if (!BWD) continue;

@@ -22,8 +22,8 @@ struct FusedArgs {
     int act;
     const void *b_gate, *b_up, *b_down;
     int residual;  // forward: there is one
-    int first;       // backward: the first chunk of rows, dy's column sums start here
-    float* sums_dy;  // backward: [CTAs][dim]
+    int first;              // backward: the first chunk of rows, the column sums start here
+    float *sums, *sums_dy;  // backward: [CTAs][4][2 hidden] of dg and du, [CTAs][dim] of dy
     uint32_t* err;
 };
 
