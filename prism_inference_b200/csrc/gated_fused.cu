@@ -10,6 +10,9 @@
 // works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3072
 // cycles of products), 80 KB backward (2850), some 30 bytes a clock; the streaming kernels of
 // gated_ffn.cu load every operand for every product and are held at the 37 to 40 that L2 gives an SM.
+// Measured: forward 522,240 x 256, hidden 1024, fp16 with residual 627 us, 1311 TFLOP/s (589 us without: the
+// 1400 that the power limit leaves a long library product), 3430 cycles a step; backward, 130,560 rows, bf16,
+// 56 us a row tile of every pair with dx, some 4500 cycles a step: MMA issue, and a stage of the ring late.
 #include <type_traits>
 
 #include "gated_fused.cuh"
