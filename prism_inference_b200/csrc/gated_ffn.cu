@@ -29,7 +29,7 @@ enum Kind : int { UP, DOWN, BACK, XW };
 constexpr int kStageA = 16384, kStageB = 16384, kStage = kStageA + kStageB;
 constexpr int kOut = 4096;  // a warp's store staging: two 32 x 32 16-bit boxes or one of fp32
 // Epilogue warps and operand stages.  BACK's epilogue works out some 20 instructions a value between
-// its TMEM loads: 16 warps hide what 8 could not (13,000 cycles a unit against the MMAs' 3072).
+// its TMEM loads: 16 warps hide what 8 could not (13,000 cycles a unit against some 3100 of MMAs).
 template <int KIND>
 struct Cfg {
     static constexpr int kEpiWarps = KIND == BACK ? 16 : 8;

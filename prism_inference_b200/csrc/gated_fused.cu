@@ -7,7 +7,7 @@
 //   backward  [g | u] and dh = dy Wd -> TMEM;  epilogue: dg, du, h -> smem, from where TMA also stores
 //             them for the weight gradients' products;  dx += dg Wg + du Wu
 // The products of step c + 1 are issued before those that need the epilogue of step c, so the tensor pipe
-// works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3072
+// works through the epilogue.  Only weights stream: 96 KB a step and SM forward (some 3100
 // cycles of products), 80 KB backward (2850), some 30 bytes a clock; the streaming kernels of
 // gated_ffn.cu load every operand for every product and are held at the 37 to 40 that L2 gives an SM.
 // Measured: forward 522,240 x 256, hidden 1024, fp16 with residual 627 us, 1311 TFLOP/s (589 us without: the
