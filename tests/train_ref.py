@@ -197,3 +197,54 @@ def gated_back(x, w, b, dy, kind, dtype):
         s, ts = rows(p, t, one)
         out[n] = (s[:, 0], ts[:, 0])
     return out
+
+
+# ---- whole numbers: sums that have to be exact ------------------------------------------------
+
+
+def whole_numbers(R, D, H, seed, device="cpu"):
+    """(x, w, b, dy) of a ReLU-gated block, as fp64 tensors, whose intermediate values are all small whole
+    numbers: x, dy and biases of -1, 0, 1; four entries of +-1 a row of w_gate and w_up, three a column of w_down
+    (fewer where places fall together).  So |g|, |u| <= 5, |dh| <= 3, |h| <= 25, |dg|, |du| <= 15, which fp16
+    and bf16 hold, and every sum stays below 25 max(R, H) < 2^24, which fp32 adds without error in any order:
+    the outputs are the exact sums, rounded once.  Signs are even-handed, so sums stay near sqrt(R) and one
+    row too many or too few shows behind that rounding."""
+    assert 25 * max(R, H) < 2 ** 24
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def small(*shape):
+        return torch.randint(-1, 2, shape, generator=g, device=device).double()
+
+    def few(rows, cols, n):
+        at = torch.randint(cols, (rows, n), generator=g, device=device)
+        sign = torch.randint(0, 2, (rows, n), generator=g, device=device).double() * 2 - 1
+        return torch.zeros((rows, cols), dtype=torch.float64, device=device).scatter_(1, at, sign)
+    return small(R, D), (few(H, D, 4), few(H, D, 4), few(H, D, 3).T.contiguous()), (small(H), small(H), small(D)), small(R, D)
+
+
+def relu_gated(x, w, b, residual):
+    return (x @ w[0].T + b[0]).clamp(min=0) * (x @ w[1].T + b[1]) @ w[2].T + b[2] + residual
+
+
+def relu_gated_back(x, w, b, dy):
+    """{name: gradient} in 64 bits."""
+    g, u, dh = x @ w[0].T + b[0], x @ w[1].T + b[1], dy @ w[2]
+    a, du, dg = g.clamp(min=0), dh * g.clamp(min=0), dh * u * (g > 0)
+    return {"dx": dg @ w[0] + du @ w[1], "dw_gate": dg.T @ x, "dw_up": du.T @ x, "dw_down": dy.T @ (a * u),
+            "db_gate": dg.sum(0), "db_up": du.sum(0), "db_down": dy.sum(0)}
+
+
+def bias_grads(x, w, b, dy, kind):
+    """{name: (bias gradient, tolerance)} where the rows' values are summed in fp32 before any rounding to 16
+    bits: 32 rows by butterfly, then a chain of the blocks of at most R / 16 additions, then 32 + 32 partial sums."""
+    x, dy, (wg, wu, wd) = x.double(), dy.double(), (v.double() for v in w)
+    g, v, t_u, a, t_a, d, t_d = _hidden(x, wg, wu, b[0].double(), b[1].double(), kind)
+    dh = dy @ wd
+    t_dh = 2 * (dy.shape[1] + 2) * U32 * (dy.abs() @ wd.abs())
+    du, dg = dh * a, dh * v * d
+    dha, va, da = dh.abs() + t_dh, v.abs() + t_u, d.abs() + t_d
+    t_du = t_dh * (a.abs() + t_a) + dh.abs() * t_a + 2 * U32 * du.abs()
+    t_dg = t_dh * va * da + dha * t_u * da + dha * va * t_d + 4 * U32 * dg.abs()
+    k = (x.shape[0] / 16 + 5 + 64) * U32
+    return {n: (p.sum(0), (t + k * (p.abs() + t)).sum(0))
+            for n, p, t in (("db_gate", dg, t_dg), ("db_up", du, t_du), ("db_down", dy, torch.zeros_like(dy)))}
