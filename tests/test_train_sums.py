@@ -45,3 +45,15 @@ def test_sums_of_rounded_rows_show(kind):
         ref.check(rows.float().sum(0).bfloat16(), *want[n], n)
         with pytest.raises(AssertionError):
             ref.check(rows.bfloat16().double().sum(0).bfloat16(), *want[n], n)
+
+
+def test_vectorised_generator():
+    for rng in ((0, 0), (0xDEADBEEF12345678, 0xF00000000000000A), (-5, -1)):
+        for t in (1, 20000, 65535):
+            assert torch.equal(ref.kept(rng, 0, 1001, t), ref.draws(rng, 1001) >= t)
+            assert torch.equal(ref.kept(rng, 800, 201, t), (ref.draws(rng, 1001) >= t)[800:])
+    # a counter above 32 bits: the high word
+    c = 2 ** 33 + 3
+    words = ref.philox_block([c & ref.M32, c >> 32, 7, 0], [9, 0])
+    bits = torch.tensor([v for w in words for v in (w & 0xFFFF, w >> 16)])
+    assert torch.equal(ref.kept((9, 7), 8 * c, 8, 30000), bits >= 30000)

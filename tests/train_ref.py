@@ -248,3 +248,24 @@ def bias_grads(x, w, b, dy, kind):
     k = (x.shape[0] / 16 + 5 + 64) * U32
     return {n: (p.sum(0), (t + k * (p.abs() + t)).sum(0))
             for n, p, t in (("db_gate", dg, t_dg), ("db_up", du, t_du), ("db_down", dy, torch.zeros_like(dy)))}
+
+
+# ---- the generator on whole tensors ------------------------------------------------------------
+
+
+def kept(rng, first, n, threshold, device="cpu"):
+    """Which of the elements first .. first + n - 1 dropout keeps (first: a multiple of 8), as one tensor
+    computation: products of 32-bit words in int64, split at 16 bits."""
+    blocks = first // 8 + torch.arange((n + 7) // 8, device=device)
+    c = [blocks & M32, blocks >> 32, torch.full_like(blocks, int(rng[1]) & M32), torch.full_like(blocks, int(rng[1]) >> 32 & M32)]
+    k = [int(rng[0]) & M32, int(rng[0]) >> 32 & M32]
+
+    def wide(m, v):  # (high, low) words of m v
+        low, high = m * (v & 0xFFFF), m * (v >> 16)
+        high = high + (low >> 16)
+        return high >> 16, (high & 0xFFFF) << 16 | (low & 0xFFFF)
+    for _ in range(10):
+        (h0, l0), (h1, l1) = wide(0xD2511F53, c[0]), wide(0xCD9E8D57, c[2])
+        c = [h1 ^ c[1] ^ k[0], l1, h0 ^ c[3] ^ k[1], l0]
+        k = [(k[0] + 0x9E3779B9) & M32, (k[1] + 0xBB67AE85) & M32]
+    return (torch.stack([w >> s & 0xFFFF for w in c for s in (0, 16)], 1).reshape(-1)[:n] >= threshold)
