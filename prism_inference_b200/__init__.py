@@ -87,11 +87,16 @@ def _I64():
 
 # These run on every call of the operators below, whose smallest calls take less time than their
 # checks: few attribute look-ups (a tensor's shape, device and so on are objects made anew each time).
+_MAX32 = 2 ** 31 - 1  # the params' fields for sizes; ctypes drops the bits above without a word
+
+
 def _rows(t, name: str):
     """(rows, dim, row stride) of a tensor [..., dim] whose last dimension is consecutive in memory."""
     shape = t.shape
     if len(shape) == 2:
         rows, dim = shape
+        if dim > _MAX32:
+            raise ValueError(f"{name}: {dim} columns, 2^31 - 1 at most (as rows of fewer columns any number of elements)")
         stride, last = t.stride()
         if last != 1 and dim > 1:
             raise ValueError(f"{name}: the last dimension is not consecutive in memory")
@@ -99,6 +104,8 @@ def _rows(t, name: str):
     if len(shape) < 1 or (shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name}: the last dimension is not consecutive in memory")
     dim = shape[-1]
+    if dim > _MAX32:
+        raise ValueError(f"{name}: {dim} columns, 2^31 - 1 at most (as rows of fewer columns any number of elements)")
     rows, stride = t.numel() // max(1, dim), dim
     if not t.is_contiguous():
         try:
@@ -308,6 +315,8 @@ class Prism:
         if activation not in abi.ACTIVATIONS:
             raise ValueError(f"activation {activation!r}: one of {', '.join(abi.ACTIVATIONS)}")
         hidden = w_gate.shape[0]
+        if hidden > _MAX32:
+            raise ValueError(f"w_gate: {hidden} rows, 2^31 - 1 at most")
         w = GatedWeights(_flat(w_gate, "w_gate", (hidden, dim), dt, dev), _flat(b_gate, "b_gate", (hidden,), dt, dev),
                          _flat(w_up, "w_up", (hidden, dim), dt, dev), _flat(b_up, "b_up", (hidden,), dt, dev),
                          _flat(w_down, "w_down", (dim, hidden), dt, dev), _flat(b_down, "b_down", (dim,), dt, dev))
