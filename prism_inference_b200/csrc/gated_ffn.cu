@@ -703,7 +703,8 @@ int check_rows(const char* who, const char* name, const void* t, int64_t stride,
     if (rows > 1 && stride < dim) return fail(PRISM_E_ARG, "%s: %s_stride %lld below dim %d", who, name, (long long)stride, dim);
     if (((uintptr_t)t & 15) || (rows > 1 && stride % 8))
         return fail(PRISM_E_ALIGN, "%s: %s and its stride have to be multiples of 16 bytes", who, name);
-    if (rows > 1 && stride > (int64_t)1 << 36) return fail(PRISM_E_RANGE, "%s: %s_stride %lld", who, name, (long long)stride);
+    if (rows > 1 && (stride > (int64_t)1 << 36 || !extent_ok(rows, stride)))
+        return fail(PRISM_E_RANGE, "%s: %s_stride %lld", who, name, (long long)stride);
     return PRISM_OK;
 }
 int check_weight(const char* who, const char* name, const void* t, bool needed, int align = 16) {

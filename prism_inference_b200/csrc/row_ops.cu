@@ -652,8 +652,9 @@ int check_stride(const char* who, const char* name, const void* t, int64_t strid
     if ((uintptr_t)t % es) return fail(PRISM_E_ALIGN, "%s: %s is not aligned to its type", who, name);
     if (rows > 1 && stride < dim)
         return fail(PRISM_E_ARG, "%s: %s_stride %lld below dim %d", who, name, (long long)stride, dim);
-    if (rows > 1 && stride > (int64_t)1 << 40) return fail(PRISM_E_RANGE, "%s: %s_stride %lld", who, name, (long long)stride);
     if (rows > (int64_t)1 << 40) return fail(PRISM_E_RANGE, "%s: rows %lld", who, (long long)rows);
+    if (rows > 1 && (stride > (int64_t)1 << 40 || !extent_ok(rows, stride)))
+        return fail(PRISM_E_RANGE, "%s: %s_stride %lld", who, name, (long long)stride);
     return PRISM_OK;
 }
 // outputs may be an input itself (same address and stride), never share bytes with it otherwise

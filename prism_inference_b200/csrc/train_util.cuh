@@ -69,6 +69,9 @@ inline bool dtype_known(int dtype) {
     return dtype == PRISM_DTYPE_F16 || dtype == PRISM_DTYPE_BF16 || dtype == PRISM_DTYPE_F32;
 }
 
+// Offsets of a tensor's rows in elements: far from what 64 bits hold in bytes, also beside an address
+inline bool extent_ok(int64_t rows, int64_t stride) { return rows <= 1 || stride <= ((int64_t)1 << 60) / rows; }
+
 // Do two tensors of `rows` rows of `dim` values share a byte?  Column slices of one wider buffer
 // (same stride, disjoint column ranges) do not; two tensors whose byte ranges meet with unlike
 // strides count as sharing.
