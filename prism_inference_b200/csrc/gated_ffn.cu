@@ -957,13 +957,16 @@ extern "C" int prism_gated_ffn_backward(prism_ctx* ctx, const prism_gated_params
         (rc = check_weight(who, "dw_down", d->dw_down, false, 2)) || (rc = check_weight(who, "db_gate", d->db_gate, false, 2)) ||
         (rc = check_weight(who, "db_up", d->db_up, false, 2)) || (rc = check_weight(who, "db_down", d->db_down, false, 2)))
         return rc;
+    const size_t nw = (size_t)p->hidden * p->dim * 2;
+    const struct { void* t; size_t n; } all[6] = {{d->dw_gate, nw}, {d->dw_up, nw}, {d->dw_down, nw},
+                                                  {d->db_gate, (size_t)p->hidden * 2}, {d->db_up, (size_t)p->hidden * 2},
+                                                  {d->db_down, (size_t)p->dim * 2}};
+    for (int i = 0; i < 6; ++i)
+        for (int j = 0; j < i; ++j)
+            if (bytes_overlap(all[i].t, all[i].n, all[j].t, all[j].n)) return fail(PRISM_E_ARG, "%s: two gradients overlap", who);
     DeviceGuard g(ctx->device);
     cudaStream_t s = as_stream(stream);
     if (p->rows == 0) {  // no rows: the sums are zero
-        const size_t nw = (size_t)p->hidden * p->dim * 2;
-        const struct { void* t; size_t n; } all[6] = {{d->dw_gate, nw}, {d->dw_up, nw}, {d->dw_down, nw},
-                                                      {d->db_gate, (size_t)p->hidden * 2}, {d->db_up, (size_t)p->hidden * 2},
-                                                      {d->db_down, (size_t)p->dim * 2}};
         for (const auto& t : all)
             if (t.t && (rc = cuda_rc(cudaMemsetAsync(t.t, 0, t.n, s), who))) return rc;
         return PRISM_OK;

@@ -691,6 +691,8 @@ extern "C" int prism_layer_norm(prism_ctx* ctx, const prism_norm_params* p, cons
         return rc;
     if (bad_alias(y, p->y_stride, x, p->x_stride, p->rows, p->dim, es))
         return fail(PRISM_E_ARG, "prism_layer_norm: y overlaps x");
+    if (bytes_overlap(mean, (size_t)p->rows * 4, rstd, (size_t)p->rows * 4))
+        return fail(PRISM_E_ARG, "prism_layer_norm: mean and rstd overlap");
     DeviceGuard g(ctx->device);
     const int64_t xs = p->rows > 1 ? p->x_stride : p->dim, ys = p->rows > 1 ? p->y_stride : p->dim;
     NormArgs a{x, weight, bias, y, mean, rstd, p->rows, xs, ys, p->dim,
@@ -730,9 +732,10 @@ extern "C" int prism_layer_norm_backward(prism_ctx* ctx, const prism_norm_params
         (rc = check_param(who, "dbias", dbias, p->param_dtype)) || (rc = check_param(who, "mean", mean, PRISM_DTYPE_F32)) ||
         (rc = check_param(who, "rstd", rstd, PRISM_DTYPE_F32)))
         return rc;
+    const size_t n = (size_t)p->dim * dtype_bytes(p->param_dtype);
+    if (bytes_overlap(dweight, n, dbias, n)) return fail(PRISM_E_ARG, "%s: dweight and dbias overlap", who);
     DeviceGuard g(ctx->device);
     if (p->rows == 0) {  // no rows: the sums are zero
-        const size_t n = (size_t)p->dim * dtype_bytes(p->param_dtype);
         if (dweight && (rc = cuda_rc(cudaMemsetAsync(dweight, 0, n, as_stream(stream)), who))) return rc;
         if (dbias && (rc = cuda_rc(cudaMemsetAsync(dbias, 0, n, as_stream(stream)), who))) return rc;
         return PRISM_OK;

@@ -72,6 +72,12 @@ inline bool dtype_known(int dtype) {
 // Offsets of a tensor's rows in elements: far from what 64 bits hold in bytes, also beside an address
 inline bool extent_ok(int64_t rows, int64_t stride) { return rows <= 1 || stride <= ((int64_t)1 << 60) / rows; }
 
+// Do two blocks of memory of na and nb bytes share one?
+inline bool bytes_overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+    return a && b && pa < pb + nb && pb < pa + na;
+}
+
 // Do two tensors of `rows` rows of `dim` values share a byte?  Column slices of one wider buffer
 // (same stride, disjoint column ranges) do not; two tensors whose byte ranges meet with unlike
 // strides count as sharing.

@@ -23,3 +23,32 @@ def test_extents_beyond_64_bits_are_refused(lib, ctx, call, names):  # noqa: F81
     for n in names.split():
         for rows, stride in ((1 << 40, 1 << 36), (1 << 30, 1 << 36), (1 << 40, 1 << 23)):
             assert call(lib, ctx, **{"rows": rows, "ws_bytes": 1 << 62, f"{n}_stride": stride}) == RANGE, (n, rows, stride)
+
+
+GRADS = ("dw_gate", "db_gate", "dw_up", "db_up", "dw_down", "db_down")
+
+
+@pytest.mark.parametrize("rows", [0, 16])
+@pytest.mark.parametrize("i,j", [(i, j) for j in range(6) for i in range(j)])
+def test_gradients_that_share_memory_are_refused(lib, ctx, rows, i, j):  # noqa: F811
+    """One address for two gradients, or the second beginning in the first's last value (dim 64, hidden 128, fp16)."""
+    sizes = {"dw_gate": 64 * 128, "db_gate": 128, "dw_up": 64 * 128, "db_up": 128, "dw_down": 64 * 128, "db_down": 64}
+    a, b = GRADS[i], GRADS[j]
+    for first, second in ((a, b), (b, a)):
+        for off in (0, 2 * sizes[first] - 2):
+            assert gated_back(lib, ctx, rows=rows, **{first: at(50), second: at(50) + off}) == abi.PRISM_E_ARG
+            assert b"overlap" in lib.prism_last_error_string()
+        if rows:  # side by side in one buffer
+            assert gated_back(lib, ctx, rows=rows, **{first: at(50), second: at(50) + 2 * sizes[first]}) == CUDA
+
+
+def test_statistics_and_parameter_gradients_that_share_memory_are_refused(lib, ctx):  # noqa: F811
+    for off in (0, 60, -60):
+        assert norm(lib, ctx, mean=at(50), rstd=at(50) + off) == abi.PRISM_E_ARG and b"overlap" in lib.prism_last_error_string()
+    assert norm(lib, ctx, mean=at(50), rstd=at(50) + 64) == CUDA
+    for rows in (0, 16):
+        for off in (0, 252, -252):  # dim 64, fp32
+            assert norm_back(lib, ctx, rows=rows, dweight=at(50), dbias=at(50) + off) == abi.PRISM_E_ARG
+            assert b"overlap" in lib.prism_last_error_string()
+    assert norm_back(lib, ctx, dweight=at(50), dbias=at(50) + 256) == CUDA
+    assert norm_back(lib, ctx, dweight=None, dbias=at(50)) == CUDA
