@@ -53,7 +53,7 @@ struct Maps {
 struct Args {
     int rows, dim, hidden;      // rows of this chunk
     int m_tiles, n_tiles;       // 256-row tiles; column tiles (128 hidden for UP / BACK, bn else)
-    int bn;                     // N of an output tile over dim: 256 or 128
+    int bn;                     // N of an output tile over dim: 256 (128: XW's dW tiles where dim <= 128)
     int units, x_units;         // XW: the first x_units are dx tiles, the others dW tiles
     int w_each[2];              // XW: dW tiles a pair takes, where it has one dx tile more than the others [1] or not
     int w_tiles, k_per, k_all;  // XW: 256-row tiles of one weight's hidden axis; row blocks a split, in all
@@ -780,7 +780,7 @@ int forward(const prism_ctx* ctx, const prism_gated_params* p, const prism_gated
         a.residual = residual ? static_cast<const T*>(residual) + r0 * rs : nullptr;
         a.residual_stride = rs;
         a.err = ctx->err;
-        a.bn = p->dim <= 128 ? 128 : 256;
+        a.bn = 256;
         a.m_tiles = (rows + 255) / 256;
         a.n_tiles = (p->hidden + 127) / 128;
         a.units = a.m_tiles * a.n_tiles;
