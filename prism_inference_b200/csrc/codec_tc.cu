@@ -46,12 +46,11 @@
 // beside their weights and staging tiles; 4 with streamed weights, whose B K-blocks share the
 // stage).  Every wait is bounded (common.cuh); on timeout the CTA sets the context's error word and
 // winds down.
-#include <cudaTypedefs.h>
-
 #include <mutex>
 
 #include "common.cuh"
 #include "host_util.h"
+#include "tensor_map.cuh"
 
 namespace prism {
 namespace {
@@ -725,18 +724,6 @@ __global__ void pixelshuffle_kernel(const __half* in, __half* rgb, int rw, int r
         const float v = __half2float(in[(int64_t)(c * sc * sc + sub) * rpx + at]);
         rgb[c * dpx + (int64_t)oy * dw + ox] = __float2half_rn(__fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-v))));
     }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
-    return fn;
 }
 
 // Per-context scratch of the codec passes: the repacked weights of each kind whose matrix is

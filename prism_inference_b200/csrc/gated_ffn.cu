@@ -14,12 +14,11 @@
 //   BACK  dh = dy Wd and [g | u] again from x -> dg, du, h, and the bias gradients' sums on the way
 //   XW    dx tiles and dW tiles (split over rows) in one launch: neither fills the GPU alone
 // Rows go through in chunks, so the scratch memory stays bounded.
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 
 #include "gated_fused.cuh"
 #include "gated_small.cuh"
+#include "tensor_map.cuh"
 
 namespace prism {
 namespace {
@@ -67,11 +66,6 @@ struct Args {
     int64_t residual_stride;
     uint32_t* err;
 };
-
-template <typename T>
-PRISM_DEV float ld_bias(const void* b, int i, int n) {
-    return b && i < n ? to_f32(static_cast<const T*>(b)[i]) : 0.0f;
-}
 
 // one unit of work, the same on every role
 struct Unit {
@@ -128,13 +122,6 @@ struct Walk {
         return x_units + (i < w_all ? i * pairs + pair : w_all * pairs + (i - w_all) * (pairs - more) + pair - more);
     }
 };
-
-// A 32 x 32 box of a warp's rows: this lane's row as 16 packed pairs into 64-byte swizzled rows.
-PRISM_DEV void stage_row64(unsigned char* buf, int lane, const uint32_t (&v)[16]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-}
 
 template <typename T, int ACT>
 PRISM_DEV void gate_cols(const uint32_t (&g)[32], const uint32_t (&u)[32], const float* bg, const float* bu, uint32_t (&out)[16]) {
@@ -584,23 +571,6 @@ __global__ void __launch_bounds__(256)
 // ---- host ------------------------------------------------------------------------------------------
 
 #define fail prism::set_error
-
-inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
-int cuda_rc(cudaError_t e, const char* what) {
-    return e == cudaSuccess ? PRISM_OK : fail(PRISM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
-    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
-}
 
 // [planes][rows][cols] with `stride` elements a row; box {box_cols, box_rows, 1}
 int make_map(CUtensorMap* m, const void* base, int dtype, int64_t cols, int64_t rows, int64_t planes, int64_t stride,

@@ -52,18 +52,6 @@ struct Bars {
     int abort;
 };
 
-template <typename T>
-PRISM_DEV float ld_bias(const void* b, int i, int n) {
-    return b && i < n ? to_f32(static_cast<const T*>(b)[i]) : 0.0f;
-}
-
-// A 32 x 32 box of a warp's rows: this lane's row as 16 packed pairs into 64-byte swizzled rows.
-PRISM_DEV void stage_row64(unsigned char* buf, int lane, const uint32_t (&v)[16]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-}
-
 template <typename T, int ACT>
 PRISM_DEV void gate32(const uint32_t (&g)[32], const uint32_t (&u)[32], const float* bg, const float* bu, uint32_t (&h)[16]) {
 #pragma unroll

@@ -106,6 +106,18 @@ PRISM_DEV uint32_t idesc_pair(int M, int N, int bf16, int a_mn, int b_mn) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+// ---- epilogues ------------------------------------------------------------------------------
+template <typename T>
+PRISM_DEV float ld_bias(const void* b, int i, int n) {
+    return b && i < n ? to_f32(static_cast<const T*>(b)[i]) : 0.0f;
+}
+
+// A 32 x 32 box of a warp's rows: this lane's row as 16 packed pairs into 64-byte swizzled rows.
+PRISM_DEV void stage_row64(unsigned char* buf, int lane, const uint32_t (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(buf + sw64_off(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
 // ---- the gate ----------------------------------------------------------------------------------
 // 1 / (1 + 2^-t): both hardware approximations are good to about 2^-22, far under the 16-bit rounding
 // that follows (tanh.approx's 2^-11 would double the error of an fp16 result).

@@ -594,11 +594,6 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs a) {
 
 #define fail prism::set_error
 
-inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
-int cuda_rc(cudaError_t e, const char* what) {
-    return e == cudaSuccess ? PRISM_OK : fail(PRISM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
 constexpr int kNormMaxDim = 16384;
 constexpr int kBackCtasPerSm = 2;  // at most: sizes the workspace
 

@@ -7,7 +7,6 @@
 //  * prism_stack_*: the whole stack over a batch of frames, with the weights repacked
 //    once into aligned device arrays for TMA and the per-expert dispatch loop
 //    replaced by route (route_kernels.cu) + one grouped tcgen05 GEMM (tc_ffn.cu).
-#include <cudaTypedefs.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -22,6 +21,7 @@
 #include "pass_kernels.cuh"
 #include "route_kernels.cuh"
 #include "tc_ffn.cuh"
+#include "tensor_map.cuh"
 
 using namespace prism;
 
@@ -53,21 +53,9 @@ namespace {
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
-    return fn;
-}
-
 // 2-D fp16 row-major [rows][cols] tensor, box [box_rows][64] with 128-byte swizzle.
 int make_map_2d(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-    auto fn = encode_fn();
+    auto fn = encode_tiled();
     if (!fn) return fail(PRISM_E_CUDA, "cuTensorMapEncodeTiled is not available");
     if (((uintptr_t)base & 15) || (cols * 2) % 16) return fail(PRISM_E_ALIGN, "tensor map base/stride not 16-byte aligned");
     cuuint64_t dims[2] = {cols, rows};
@@ -85,7 +73,7 @@ int make_map_2d(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, 
 // one load brings box_rows rows at their full K, one [box_rows][128 B] swizzled tile per
 // 64-wide K-block.
 int make_map_kb3d(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-    auto fn = encode_fn();
+    auto fn = encode_tiled();
     if (!fn) return fail(PRISM_E_CUDA, "cuTensorMapEncodeTiled is not available");
     if (((uintptr_t)base & 15) || cols % 64) return fail(PRISM_E_ALIGN, "K-block weight map: bad base or width");
     cuuint64_t dims[3] = {64, rows, cols / 64};
@@ -110,7 +98,7 @@ std::vector<uint16_t> kb_major(const std::vector<uint16_t>& m, size_t rows, size
 // 4-D fp16 activation tensor (C, X=W, Y=H, F) HWC per frame, box {64, 8, 8, 1}, 128B swizzle:
 // one box is one 8x8 window, 64 channels, rows in window-slot order.
 int make_map_act4d(CUtensorMap* m, const void* base, int C, int W, int H, int F) {
-    auto fn = encode_fn();
+    auto fn = encode_tiled();
     if (!fn) return fail(PRISM_E_CUDA, "cuTensorMapEncodeTiled is not available");
     if ((uintptr_t)base & 15) return fail(PRISM_E_ALIGN, "activation buffer not 16-byte aligned");
     cuuint64_t dims[4] = {(cuuint64_t)C, (cuuint64_t)W, (cuuint64_t)H, (cuuint64_t)F};

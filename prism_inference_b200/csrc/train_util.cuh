@@ -64,6 +64,11 @@ inline cudaError_t allow_smem(K kernel, int bytes, int device, std::atomic<uint6
     return e;
 }
 
+inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+inline int cuda_rc(cudaError_t e, const char* what) {
+    return e == cudaSuccess ? PRISM_OK : set_error(PRISM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 inline int dtype_bytes(int dtype) { return dtype == PRISM_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_known(int dtype) {
     return dtype == PRISM_DTYPE_F16 || dtype == PRISM_DTYPE_BF16 || dtype == PRISM_DTYPE_F32;
