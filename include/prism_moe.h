@@ -238,7 +238,9 @@ int prism_ctx_status(prism_ctx* ctx, void* stream);
  * Scratch memory is the caller's too: *_workspace() says how many bytes a call with these
  * params needs (16-byte aligned, any contents, free again when the call's work has run), so
  * calls on different streams, threads or captured graphs share nothing unless the caller
- * gives them the same workspace.  The same inputs give the same bits (no atomics).
+ * gives them the same workspace.  The same inputs give the same bits: no sum's order depends on
+ * timing (what the gated backward pass adds in memory, it adds from one place an address, in one
+ * order).
  * Calls are stream-ordered, never synchronise, never allocate and can be captured into a
  * CUDA graph.  rows == 0 is a no-op (the gradients of parameters become zero).  A bounded device
  * wait of the gated kernels that gives up is reported by prism_ctx_status. */
@@ -316,7 +318,9 @@ typedef struct prism_gated_grads {
 
 /* y = w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down + residual, row by row; residual
  * nullable.  Products accumulate in fp32; the hidden values are rounded once to dtype, as the
- * operand of the last product (not for a few rows), and y once.  y must not overlap x; it may be residual itself. */
+ * operand of the last product, and y once.  For a few rows (at most 8, with (rows - 1) * dim * hidden <=
+ * 2^24) the hidden values stay in fp32: one beyond fp16's 65504 is finite there and an infinity in a
+ * larger fp16 batch.  y must not overlap x; it may be residual itself. */
 int prism_gated_ffn(prism_ctx* ctx, const prism_gated_params* p, const prism_gated_weights* w, const void* x,
                     const void* residual, void* y, void* workspace, size_t workspace_bytes, void* stream);
 /* The gradients of sum(dy * y) without the residual path (dy itself) from x and the weights: the
@@ -327,8 +331,12 @@ int prism_gated_ffn_backward(prism_ctx* ctx, const prism_gated_params* p, const 
                              const void* dy, void* dx, const prism_gated_grads* grads, void* workspace,
                              size_t workspace_bytes, void* stream);
 /* The workspace of the forward (backward = 0) or backward (1) call.  Forward: 4 hidden bytes a row for a few
- * rows (up to 8); beyond, none for dim <= 256, else 2 hidden bytes a row up to 1 GiB (rows go through in chunks).  Backward: 6 hidden bytes a row up to
- * 1 GiB, and fp32 partial sums of the gradients. */
+ * rows (as above); beyond, none for dim <= 256, else 2 hidden bytes a row of a chunk.  Backward: 6 hidden bytes
+ * a row of a chunk, and fp32 partial sums of the gradients (of the weights: 12 hidden dim bytes, a few
+ * times over while that is small).  Rows go through in chunks of as many waves (128 rows an SM, 18,944 on 148
+ * SMs) as 1 GiB holds, of one wave where it holds none: a chunk takes at most the larger of 1 GiB and
+ * a wave, which passes 1 GiB for hidden above 9440 backward (1.5 GiB at 14336, 6.9 at 65536) and above 28336
+ * forward (2.3 at 65536). */
 int prism_gated_ffn_workspace(prism_ctx* ctx, const prism_gated_params* p, int backward, size_t* bytes);
 
 /* ---- fast path: a whole stack over a batch of frames ------------------------ */

@@ -604,7 +604,7 @@ int launch(const prism_ctx* ctx, const Args& a, const Maps& m, cudaStream_t s, c
 }
 
 // Rows that go through at a time: whole waves of a row tile for every CTA pair, as many as keep
-// `row_bytes` of scratch a row within 1 GiB, one at least.  (130,560 x 256, hidden 1024, backward: 635 us
+// `row_bytes` of scratch a row within 1 GiB, one at least (also where that is more than 1 GiB).  (130,560 x 256, hidden 1024, backward: 635 us
 // by single waves, whose scratch half stays in L2, 559 us in one piece: launches and their first
 // loads cost more than L2 gives.)
 int64_t chunk_rows(const prism_ctx* ctx, int64_t rows, int64_t row_bytes) {

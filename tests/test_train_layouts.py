@@ -1,10 +1,13 @@
 """Row layouts that the trainable sub-block's C entries take or refuse, beside those of test_train_refusals.py:
 without a GPU, where a call that is let through ends with the missing device."""
+import ctypes as C
+
 import pytest
 
 from prism_inference_b200 import abi
+from prism_inference_b200.abi import GatedParams
 
-from test_train_refusals import at, ctx, drop, gated, gated_back, lib, norm, norm_back  # noqa: F401
+from test_train_refusals import GATED, at, ctx, drop, gated, gated_back, lib, norm, norm_back  # noqa: F401
 
 RANGE, CUDA = abi.PRISM_E_RANGE, abi.PRISM_E_CUDA
 
@@ -52,3 +55,22 @@ def test_statistics_and_parameter_gradients_that_share_memory_are_refused(lib, c
             assert b"overlap" in lib.prism_last_error_string()
     assert norm_back(lib, ctx, dweight=at(50), dbias=at(50) + 256) == CUDA
     assert norm_back(lib, ctx, dweight=None, dbias=at(50)) == CUDA
+
+
+@pytest.mark.parametrize("dim", [64, 256, 264, 4096, 16384])
+@pytest.mark.parametrize("hidden", [1024, 9440, 9448, 14336, 28336, 28344, 65536])
+def test_workspace_is_what_the_header_says(lib, ctx, dim, hidden):  # noqa: F811
+    """A chunk of rows takes the larger of 1 GiB and one wave (128 rows an SM) at most, however many rows there are;
+    the gradients' partial sums come on top backward."""
+    def size(backward, rows):
+        n, p = C.c_size_t(), GatedParams(**dict(GATED, rows=rows, dim=dim, hidden=hidden))
+        assert lib.prism_gated_ffn_workspace(C.byref(ctx), C.byref(p), backward, C.byref(n)) == 0
+        return n.value
+    wave, rows = 128 * 148, 10 ** 8
+    chunk = max(1 << 30, wave * 2 * hidden)
+    assert (wave * 2 * hidden > 1 << 30) == (hidden > 28336) and (wave * 6 * hidden > 1 << 30) == (hidden > 9440)
+    assert size(0, rows) == 0 if dim <= 256 else chunk // 2 < size(0, rows) <= chunk
+    chunk = max(1 << 30, wave * 6 * hidden)
+    tiles = 3 * -(-hidden // 256) * -(-dim // 256)
+    sums = max(1, 74 // tiles) * 12 * hidden * dim + 4 * (8 * 74 * 2 * hidden + (2 * 74 + 16 * 24) * dim)
+    assert chunk // 2 < size(1, rows) <= chunk + sums + 2048
