@@ -83,10 +83,12 @@ PRISM_DEV void mbar_wait_step(uint64_t* bar, uint32_t parity, volatile int* abor
     if (!mbar_try_wait(bar, parity)) mbar_wait_spin(bar, parity, abort);
     __syncwarp();
 }
-// Arrives on an mbarrier of this CTA or its peer (a shared::cluster address).  What is handed over is
-// shared memory that the tensor core reads (made visible by fence.proxy.async before) or TMEM (by
-// tcgen05.fence), so the arrival itself carries no cluster-scope release, which costs a full memory
-// barrier: 40 -> 33 us for 8160 rows forward.
+// Arrives on an mbarrier of this CTA or its peer (a shared::cluster address), without a cluster-scope
+// release, which costs a full memory barrier: 40 -> 33 us for 8160 rows forward.  What is handed over is
+// this CTA's own shared memory, written before a fence.proxy.async and read by the tensor core alone, or
+// its TMEM, read before a tcgen05.fence.  The written memory model orders that against the other CTA's
+// waiter only by a cluster-scope release.  That the fence and this arrival are enough is practice relied on (the
+// memory that the tensor core reads is the one that the fence completed the writes to), not its guarantee.
 PRISM_DEV void mbar_arrive_pair(uint32_t bar_cluster) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
