@@ -7,12 +7,15 @@
 //   backward  [g | u] and dh = dy Wd -> TMEM;  epilogue: dg, du, h -> smem, from where TMA also stores
 //             them for the weight gradients' products;  dx += dg Wg + du Wu
 // The products of step c + 1 are issued before those that need the epilogue of step c, so the tensor pipe
-// works through the epilogue.  Only weights stream: 96 KB a step and SM forward (some 3100
-// cycles of products), 80 KB backward (2850), some 30 bytes a clock; the streaming kernels of
+// works through the epilogue.  Only weights stream: 96 KB a step and SM forward (3070 cycles of the
+// tensor pipe), 80 KB backward (2560), at that pace some 30 bytes a clock; the streaming kernels of
 // gated_ffn.cu load every operand for every product and are held at the 37 to 40 that L2 gives an SM.
 // Measured: forward 522,240 x 256, hidden 1024, fp16 with residual 627 us, 1311 TFLOP/s (589 us without: the
-// 1400 that the power limit leaves a long library product), 3430 cycles a step; backward, 130,560 rows, bf16,
-// 56 us a row tile of every pair with dx, some 4500 cycles a step: MMA issue, and a stage of the ring late.
+// 1400 that the power limit leaves a long library product); backward with dx alone, bf16, 55 us for a row
+// tile of every pair.  Steps and tensor pipe: 27 row tiles a pair forward, run for seconds, 4720 cycles a step at
+// the sampled 1410 MHz (4640 a step more for a tile more), three tiles 4800 with the pipe 64 % busy; backward
+// 6210 at 1590 MHz over 14 tiles (6170), three tiles 5810 with the pipe 44 % busy.  The rest is waits: for the ring's
+// stages, the commits between, and the epilogue that the next products' operands come from.
 #include <type_traits>
 
 #include "gated_fused.cuh"
