@@ -234,7 +234,7 @@ int prism_ctx_status(prism_ctx* ctx, void* stream);
  * consecutive in memory, rows at *_stride ELEMENTS from one another (at least dim; ignored
  * for a single row), so column slices of a wider buffer work.  An output shares memory with
  * another tensor of its call only where its entry says so.  Activations, weights and
- * gradients are fp16, bf16 or fp32 (enum prism_dtype); sums and statistics are fp32.
+ * gradients are fp16, bf16 or fp32 (enum prism_dtype); sums and statistics are fp32 or wider.
  * Scratch memory is the caller's too: *_workspace() says how many bytes a call with these
  * params needs (16-byte aligned, any contents, free again when the call's work has run), so
  * calls on different streams, threads or captured graphs share nothing unless the caller

@@ -437,30 +437,32 @@ __global__ void __launch_bounds__(kThreads, back_ctas_per_sm<FAST, T, NV>()) nor
 }
 
 // Adds the CTAs' partial sums: 32 columns a CTA, 32 threads a column over every 32nd partial, then the
-// 32 in order.
+// 32 in order.  In 64 bits: in 32 these last additions, of nearly whole sums, made up more than half of the
+// squared error (4,099 x 1,001 fp32, root mean square over the columns: 1.4e-7 against 7.2e-8), and the kernel
+// waits for its loads anyway.
 template <typename T>
 __global__ void __launch_bounds__(1024)
     norm_fold_kernel(const float* part, int n_part, int dim, void* dweight, void* dbias, int param_f32) {
-    __shared__ float red[32][33];
+    __shared__ double red[32][33];
     grid_dep_wait();
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;  // over [dweight | dbias]
-    float s = 0.0f;
+    double s = 0.0;
     if (c < 2 * dim)
         for (int p = k; p < n_part; p += 32) s += part[(int64_t)p * 2 * dim + c];
     red[k][lane] = s;
     __syncthreads();
     if (k == 0 && c < 2 * dim) {
-        s = 0.0f;
+        s = 0.0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) s += red[i][lane];
         void* dst = c < dim ? dweight : dbias;
         const int i = c < dim ? c : c - dim;
         if (dst) {
             if (param_f32)
-                static_cast<float*>(dst)[i] = s;
+                static_cast<float*>(dst)[i] = (float)s;
             else
-                static_cast<T*>(dst)[i] = from_f32<T>(s);
+                static_cast<T*>(dst)[i] = from_f32<T>((float)s);
         }
     }
 }

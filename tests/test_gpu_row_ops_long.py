@@ -128,3 +128,26 @@ def test_element_offsets_past_32_bits(prism_ctx, D):
     for p in parts:
         want, tol = ref.norm_back(x[p], w, mean[p], rstd[p], x[p], None)
         ref.check(y[p], want[0], tol[0], f"dx {p}")
+
+
+@pytest.mark.parametrize("shape", [(4099, 1001), (4099, 1000), (20000, 256)])
+def test_parameter_gradients_lose_little_to_their_sums(prism_ctx, shape):
+    """The root mean square of the sums' error over the columns.  An fp32 rounding is off by at most 2^-24 of its value,
+    evenly spread, so by 2^-24 / sqrt(3) in the mean square; independent ones add up in squares, each weighted with its partial sum's
+    share of the rows: c = rows a thread adds up (c^2 / 2 + c / 2 for each of the R / c threads of a column),
+    then p threads of a CTA (a running sum each, c p (p + 1) / 2 for each of the R / (c p) CTAs).  Then a
+    rounding to fp32, and three on each term (x - mean, the product with rstd, the fused product with dy).
+    What joins the CTAs' partial sums has no share: it adds in 64 bits."""
+    R, D = shape
+    x, dy = rand(shape, F32, 31) - 0.25, rand(shape, F32, 32) - 0.25
+    mean, rstd = torch.zeros(R, device="cuda"), torch.ones(R, device="cuda")
+    dw, db = torch.empty(D, device="cuda"), torch.empty(D, device="cuda")
+    prism_ctx.layer_norm_backward(x, None, mean, rstd, dy, torch.empty_like(x), dweight=dw, dbias=db)
+    # a team has D / 16 threads, rounded up to a power of two; one CTA of 256 threads on each of 148 SMs.  Teams of
+    # less than a warp: 32 / team of them come together by butterfly, in place of running sums
+    p = 256 // (64 if D > 512 else 16)
+    c = -(-R // (148 * p))
+    squares = ((c + 1) / 2 + (p + 1) / 2 + 1 + 3)
+    for got, want in ((dw, (dy.double() * x.double()).sum(0)), (db, dy.double().sum(0))):
+        off = float((got.double() - want).norm() / want.norm())
+        assert off < (squares / 3) ** 0.5 * ref.U32, (off, (squares / 3) ** 0.5 * ref.U32)
